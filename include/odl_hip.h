@@ -340,6 +340,33 @@ int odl_hip_softmax_ce_loss_grad_device(const float *x, const void *t, int idx_i
                                         float *device_loss2, void *host_mirror2, float *unit_gx, void *workspace,
                                         size_t workspace_bytes, void *stream);
 
+/* A Linear layer and the cross entropy of its outputs as one operator (Linear::forward, src/nn/layers/linear.cpp:80-106,
+ * then SoftmaxCrossEntropy, src/operators/loss/softmax_cross_entropy.cpp:17-111) for large vocabularies: the [N, V] logits
+ * z = x[N,K] . w + b are never stored, neither in the forward nor in the backward pass, which goes over the vocabulary in
+ * pieces. w is [K, V] as nn::Linear keeps it, or [V, K] with w_out_in != 0 (LinearOp's layout, src/operators/custom/linear.cpp,
+ * and an embedding's); b[V] may be NULL, and may hold -inf for entries that must not be predicted.
+ *   loss = 1/C * sum over the C counted rows of (log sum_v exp(z[n][v]) - z[n][t[n]])
+ * Rows whose label is ignore_index are not counted (pass a value no label has, e.g. -100, to count all): they add nothing to
+ * the loss or to a gradient, whatever x holds there, NaN included. With no counted row the loss and all gradients are 0.
+ * Unlike odl_hip_softmax_ce_loss the probability is not offset by 1e-8 before the logarithm: the loss is the exact negative
+ * log-likelihood and the gradient its derivative. Products are float32 in accuracy (each operand as two float16 numbers,
+ * three products, float32 sums). Neither call synchronises or allocates; both can be captured.
+ * forward: device_saved8[0] the loss, [1] (an int) nonzero if a label that is not ignore_index lies outside [0, V) — such a
+ * row is left out like an ignored one, the caller decides when to look —, [2] the number of counted rows, the rest and
+ * row_stats[N, 2] (base-2 logarithm of the row's largest exp(z), sum of exp(z) over that) are for the backward pass.
+ * backward: gx[N,K], gw (w's layout), gb[V], each may be NULL; the upstream gradient is read from device_gy[0] (NULL: 1).
+ * x, w, b, t, saved and row_stats are the forward call's, unchanged; outputs must not overlap inputs.
+ * N = 0 is an empty batch. N and K up to 2^20, V up to 2^30; the workspace's alignment is 16 bytes. */
+int odl_hip_linear_softmax_ce_forward(const float *x, const float *w, int w_out_in, const float *b, const void *t, int idx_is_i64,
+                                      int64_t ignore_index, int64_t N, int64_t K, int64_t V, float *device_saved8,
+                                      float *row_stats, void *workspace, size_t workspace_bytes, void *stream);
+size_t odl_hip_linear_softmax_ce_forward_workspace_bytes(int64_t N, int64_t K, int64_t V);
+int odl_hip_linear_softmax_ce_backward(const float *device_gy, const float *x, const float *w, int w_out_in, const float *b,
+                                       const void *t, int idx_is_i64, int64_t ignore_index, int64_t N, int64_t K, int64_t V,
+                                       const float *device_saved8, const float *row_stats, float *gx, float *gw, float *gb,
+                                       void *workspace, size_t workspace_bytes, void *stream);
+size_t odl_hip_linear_softmax_ce_backward_workspace_bytes(int64_t N, int64_t K, int64_t V);
+
 /* ------------------------------------------------------------------ pooling ------------------------- */
 /* Mat::max_pool2d / max_pool2d_backward (mat.h:560-578; src/mat/origin/cpu/pooling/max_pool2d.cpp:40-224).
  * idx[n,c,oh,ow] = kh*KW+kw of the first maximum (strict >, scan starts at window cell (0,0));
@@ -628,6 +655,25 @@ int odl_hip_adam_step_multi_decay(int count, const float *const *p, float *const
                                   float *const *p_out, void *stream);
 int odl_hip_sgd_step_multi_decay(int count, const float *const *p, float *const *g, const int64_t *n, float weight_decay,
                                  float lr, float *const *p_out, void *stream);
+/* Orthogonalised updates, for a matrix optimiser beside SGD and Adam (no counterpart in the reference).
+ * newton_schulz: out = X after `steps` of X <- a X + (b A + c A A) X, A = X X^T, from X0 = g / (||g||_F + eps), on the side of
+ * the shorter dimension, for `batch` dense matrices g[batch, rows, cols]. (a, b, c) = (3.4445, -4.775, 2.0315) brings the
+ * singular values to about [0.7, 1.2] in five steps. Coefficients under which they, or b A + c A A, could pass 7.5 on the way
+ * are refused. A zero matrix gives zeros; a matrix with an infinity or a NaN gives NaN. out may be g.
+ * muon_step_multi: one optimiser step over a list of matrices [host_rows[i], host_cols[i]]; equal shapes go through the same
+ * launches, up to 32 together:
+ *   buf = momentum * buf + g;  u = nesterov ? g + momentum * buf : buf;  O = newton_schulz(u)
+ *   p_out = p * (1 - lr * weight_decay) - lr * sqrt(max(1, rows / cols)) * O
+ * buf is updated in place, p_out may be p; the same buffer must not stand for two entries. Empty matrices are skipped.
+ * Sides up to 2^20, 1 to 100 steps. Neither call synchronises or allocates device memory; both can be captured. */
+int odl_hip_newton_schulz(const float *g, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c,
+                          float eps, float *out, void *workspace, size_t workspace_bytes, void *stream);
+size_t odl_hip_newton_schulz_workspace_bytes(int64_t batch, int64_t rows, int64_t cols);
+int odl_hip_muon_step_multi(int count, const float *const *p, const float *const *g, float *const *buf, const int64_t *host_rows,
+                            const int64_t *host_cols, float lr, float momentum, int nesterov, float weight_decay, int steps,
+                            float a, float b, float c, float eps, float *const *p_out, void *workspace, size_t workspace_bytes,
+                            void *stream);
+size_t odl_hip_muon_step_multi_workspace_bytes(int count, const int64_t *host_rows, const int64_t *host_cols);
 /* origin::cuda::{zeros,ones,full} (cuda/factory.cuh:23-50) */
 int odl_hip_fill(float *dst, int64_t n, float value, void *stream);
 

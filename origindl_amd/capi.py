@@ -487,6 +487,63 @@ def softmax_cross_entropy_with_unit_grad(x, t):
     return float(words[0]), int(words.view(torch.int32)[1]), gx
 
 
+# ------------------------------------------------------ output layer with its loss, large vocabularies
+def _ce_args(who, x, w, b, t, w_out_in):
+    _chk(x, "x"), _chk(w, "w")
+    if x.dim() != 2 or w.dim() != 2:
+        raise OdlInvalidArgument("%s: x must be (N, K) and w 2D, got %s and %s" % (who, tuple(x.shape), tuple(w.shape)))
+    N, K = x.shape
+    V, Kw = w.shape if w_out_in else (w.shape[1], w.shape[0])
+    if K != Kw:
+        raise OdlInvalidArgument("%s: x has %d features, w expects %d" % (who, K, Kw))
+    if b is not None and (_chk(b, "b").numel() != V or b.shape[-1] != V):
+        raise OdlInvalidArgument("%s: b must hold %d values, got shape %s" % (who, V, tuple(b.shape)))
+    t, is64 = _labels(t)
+    if t.dim() != 1 or t.shape[0] != N:
+        raise OdlInvalidArgument("%s: target must be (%d,), got %s" % (who, N, tuple(t.shape)))
+    for name, other in (("w", w), ("b", b), ("target", t)):
+        if other is not None and other.device != x.device:
+            raise OdlInvalidArgument("%s: %s is on %s, x on %s" % (who, name, other.device, x.device))
+    return N, K, V, is64
+
+
+def linear_softmax_cross_entropy(x, w, b, t, ignore_index=-100, w_out_in=False):
+    """Mean cross entropy of softmax(x . w + b) without storing the logits -> (loss, saved): loss a 0-dim device tensor,
+    saved = (words, row_stats) for the backward pass; words[1] viewed as int32 is nonzero after a label out of range (see
+    linear_softmax_cross_entropy_bad_label). w: [K, V], or [V, K] with w_out_in. Does not synchronise."""
+    N, K, V, is64 = _ce_args("linear_softmax_cross_entropy", x, w, b, t, w_out_in)
+    with torch.cuda.device(x.device):
+        saved, rows = _empty((8,)), _empty((N, 2))
+        ws, nb = _ws(lib().query("odl_hip_linear_softmax_ce_forward_workspace_bytes", N, K, V))
+        lib().call("odl_hip_linear_softmax_ce_forward", _p(x), _p(w), int(w_out_in), _p(b), _p(t), is64, int(ignore_index), N, K, V,
+                   _p(saved), _p(rows), _p(ws), nb, _stream())
+    return saved[0], (saved, rows)
+
+
+def linear_softmax_cross_entropy_bad_label(saved):
+    """Whether the forward pass met a label that is neither ignore_index nor in [0, V) (reads one word from the device)."""
+    return bool(saved[0].view(torch.int32)[1].item() != 0)
+
+
+def linear_softmax_cross_entropy_backward(gy, x, w, b, t, saved, ignore_index=-100, w_out_in=False, need_gx=True, need_gw=True,
+                                          need_gb=True):
+    """-> (gx, gw, gb), None where not asked for; gy a float32 device tensor of one element, or None for 1."""
+    N, K, V, is64 = _ce_args("linear_softmax_cross_entropy_backward", x, w, b, t, w_out_in)
+    if gy is not None and (_chk(gy, "gy").numel() != 1 or gy.device != x.device):
+        raise OdlInvalidArgument("linear_softmax_cross_entropy_backward: gy must be one element on x's device")
+    words, rows = _chk(saved[0], "saved"), _chk(saved[1], "saved")
+    if words.numel() != 8 or tuple(rows.shape) != (N, 2) or words.device != x.device or rows.device != x.device:
+        raise OdlInvalidArgument("linear_softmax_cross_entropy_backward: saved is not from a forward call with %d rows" % N)
+    with torch.cuda.device(x.device):
+        gx = _empty((N, K)) if need_gx else None
+        gw = _empty(w.shape) if need_gw else None
+        gb = _empty((V,)) if need_gb else None
+        ws, nb = _ws(lib().query("odl_hip_linear_softmax_ce_backward_workspace_bytes", N, K, V))
+        lib().call("odl_hip_linear_softmax_ce_backward", _p(gy), _p(x), _p(w), int(w_out_in), _p(b), _p(t), is64, int(ignore_index), N, K,
+                   V, _p(words), _p(rows), _p(gx), _p(gw), _p(gb), _p(ws), nb, _stream())
+    return gx, gw, gb
+
+
 # ----------------------------------------------------------------------------------------- pooling
 def max_pool2d(x, kernel_size, stride, pad, with_indices=True):
     _chk(x, "x")
@@ -1058,6 +1115,47 @@ def axpy_multi(alpha, xs, ys):
             raise OdlInvalidArgument("axpy_multi: shape mismatch")
     lib().call("odl_hip_axpy_multi", len(xs), float(np.float32(alpha)), _ptr_array(xs), _ptr_array(ys), _size_array(xs),
                _stream())
+
+
+def newton_schulz(g, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """The matrix g [rows, cols] — or each of g [batch, rows, cols] — with its singular values brought towards 1 by `steps`
+    Newton-Schulz products X <- aX + (bA + cAA)X, A = X X^T, from g / (||g||_F + eps)."""
+    _chk(g, "g")
+    if g.dim() not in (2, 3):
+        raise OdlInvalidArgument("newton_schulz: g must be 2D or 3D, got %s" % (tuple(g.shape),))
+    batch, rows, cols = (1,) + tuple(g.shape) if g.dim() == 2 else tuple(g.shape)
+    a, b, c = (float(v) for v in coefficients)
+    with torch.cuda.device(g.device):
+        out = _empty(g.shape)
+        ws, nb = _ws(lib().query("odl_hip_newton_schulz_workspace_bytes", batch, rows, cols))
+        lib().call("odl_hip_newton_schulz", _p(g), batch, rows, cols, int(steps), a, b, c, float(eps), _p(out), _p(ws), nb, _stream())
+    return out
+
+
+def muon_step_multi(ps, gs, bufs, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
+                    coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """One orthogonalised-momentum step over a list of matrices: bufs[i] = momentum * bufs[i] + gs[i] in place, returns the new
+    parameters p * (1 - lr * weight_decay) - lr * sqrt(max(1, rows / cols)) * newton_schulz(update)."""
+    if not (len(ps) == len(gs) == len(bufs)):
+        raise OdlInvalidArgument("muon_step_multi: lists of different lengths")
+    for p, g, buf in zip(ps, gs, bufs):
+        for x in (p, g, buf):
+            if _chk(x, "muon_step_multi operand").dim() != 2 or x.shape != p.shape or x.device != ps[0].device:
+                raise OdlInvalidArgument("muon_step_multi: parameter, gradient and buffer must be matrices of one shape on one device")
+    if len({buf.data_ptr() for buf in bufs if buf.numel()}) != _builtins.sum(1 for buf in bufs if buf.numel()):
+        raise OdlInvalidArgument("muon_step_multi: a buffer stands for two entries")
+    if not ps:
+        return []
+    n = len(ps)
+    rows = (ctypes.c_int64 * n)(*[int(p.shape[0]) for p in ps])
+    cols = (ctypes.c_int64 * n)(*[int(p.shape[1]) for p in ps])
+    a, b, c = (float(v) for v in coefficients)
+    with torch.cuda.device(ps[0].device):
+        outs = [_empty(p.shape) for p in ps]
+        ws, nb = _ws(lib().query("odl_hip_muon_step_multi_workspace_bytes", n, rows, cols))
+        lib().call("odl_hip_muon_step_multi", n, _ptr_array(ps), _ptr_array(gs), _ptr_array(bufs), rows, cols, float(lr), float(momentum),
+                   int(nesterov), float(weight_decay), int(steps), a, b, c, float(eps), _ptr_array(outs), _p(ws), nb, _stream())
+    return outs
 
 
 def fill(shape, value):

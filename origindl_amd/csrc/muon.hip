@@ -1,0 +1,472 @@
+// Orthogonalised updates: Newton-Schulz steps on a matrix (or a list of equal ones), and the optimiser step around them.
+//
+//   X0 = U / (||U||_F + eps), transposed if it has more rows than columns (m <= n from here on)
+//   X <- a X + (b A + c A A) X,  A = X X^T        `steps` times
+//   U: the gradient; in the optimiser step the momentum buf <- mu buf + g, or g + mu buf (Nesterov)
+//   p <- p (1 - lr * weight_decay) - lr * sqrt(max(1, rows / cols)) * X
+//
+// What bounds it: three products a step, 2m^2 n + 2m^3 + 2m^2 n operations, of which the two symmetric ones need only half of
+// their tiles. They run as three float16 products each (split_gemm.h); X, A and b A + c A A live only as operands of
+// those, between launches in L2 and the memory-side cache. Every epilogue writes its result as the next product's operands: X
+// as rows of m (for X X^T) and as rows of n (for B X), the symmetric ones with their mirror image. The last one writes X, or
+// applies it to the parameter.
+//
+// Singular values of X stay under max |f| on [0, 1], f(s) = a s + b s^3 + c s^5 (1.21 for the usual coefficients), so all
+// operands are scaled by the same 2^13: float16 holds 8 * 2^13, and coefficients that lead past 7.5 are refused.
+#include <cmath>
+#include <vector>
+
+#include "split_gemm.h"
+
+namespace
+{
+using namespace odl::split;
+
+constexpr int kBlock     = 256;
+constexpr float kScale   = 8192.f;
+constexpr double kMost   = 7.5;
+constexpr int kGroup     = 32;  // matrices per launch
+
+struct Matrices  // one launch's matrices: all [rows, cols]
+{
+    const float *g[kGroup];
+    float *buf[kGroup];    // null: U is the gradient itself
+    const float *p[kGroup];
+    float *out[kGroup];    // X, or the new parameter where p is not null
+    int64_t rows, cols;
+    float momentum;
+    int nesterov;
+
+};
+
+// U's element i; buf holds the new momentum already
+struct Update
+{
+    const float *g, *buf;
+    float momentum;
+    int nesterov;
+    __device__ float operator()(int64_t i) const
+    {
+        if (!buf)
+            return g[i];
+        return nesterov ? g[i] + momentum * buf[i] : buf[i];
+    }
+};
+
+// buf <- mu buf + g, and the partial sums of U's squares, in 64 bits: the norm's error is common to all of X, and the steps
+// amplify it
+__global__ __launch_bounds__(kBlock) void muon_norm_kernel(const Matrices a, double *sums)
+{
+    __shared__ double part[4];
+    const int z = blockIdx.y;
+    const int64_t n = a.rows * a.cols;
+    float *buf = a.buf[z];
+    const Update u{a.g[z], buf, a.momentum, a.nesterov};
+    double s = 0.0;
+    for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (int64_t)gridDim.x * kBlock)
+    {
+        if (buf)
+            buf[i] = buf[i] * a.momentum + u.g[i];
+        const double v = (double)u(i);
+        s += v * v;
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0)
+        part[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        sums[(int64_t)z * gridDim.x + blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
+}
+
+struct ScaledUpdate
+{
+    Update u;
+    int64_t cols;
+    double factor;
+    __device__ float operator()(int64_t r, int64_t c) const { return (float)((double)u(r * cols + c) * factor); }
+};
+
+// X0 as panels: r has the matrix's rows as rows, t its columns
+__global__ __launch_bounds__(kBlock) void muon_prepare_kernel(const Matrices a, const double *sums, int parts, double eps, Panel r, Panel t,
+                                                              int64_t batch_bytes)
+{
+    __shared__ float tile[64][65];
+    __shared__ double part[4];
+    const int z = blockIdx.z;
+    double s = 0.0;
+    for (int i = threadIdx.x; i < parts; i += kBlock)
+        s += sums[(int64_t)z * parts + i];
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+        s += __shfl_xor(s, o, 64);
+    if ((threadIdx.x & 63) == 0)
+        part[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = (part[0] + part[1]) + (part[2] + part[3]);
+    r.base += z * batch_bytes, t.base += z * batch_bytes;
+    split_tile(ScaledUpdate{{a.g[z], a.buf[z], a.momentum, a.nesterov}, a.cols, (double)kScale / (sqrt(s) + eps)}, a.rows, a.cols, (int64_t)blockIdx.y * 64, (int64_t)blockIdx.x * 64, r, t, tile);
+}
+
+// the accumulator block as rows of the other side: through the wave's scratch
+__device__ inline void store_mirror(const Panel &p, int64_t rb, int64_t cb, int lane, const f32x16 &c, float *scratch)
+{
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+        scratch[(16 * (e >> 3) + 8 * (lane >> 5) + (e & 7)) * 33 + (lane & 31)] = c[e];
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+    {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            v[e] = scratch[(lane & 31) * 33 + 16 * h + 8 * (lane >> 5) + e];
+        store_fragment(p, rb, cb * 2 + h, lane, v);
+    }
+    __builtin_amdgcn_wave_barrier();
+}
+
+// c[8h + e] <- own * acc + before * prev at the block's place in a panel of the column side, kept times kScale
+__device__ inline void combine(f32x16 &c, const Panel &prev, int64_t cb, int64_t rb, int lane, float own, float before)
+{
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+    {
+        float v[8];
+        load_fragment(prev, cb, rb * 2 + h, lane, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            c[8 * h + e] = fmaf(own, c[8 * h + e], before * v[e]);
+    }
+}
+
+__device__ inline void store_columns(const Panel &p, int64_t cb, int64_t rb, int lane, const f32x16 &c)
+{
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+    {
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            v[e] = c[8 * h + e];
+        store_fragment(p, cb, rb * 2 + h, lane, v);
+    }
+}
+
+// A = X X^T (prev null), or b A + c A A: symmetric, computed for tile row <= tile column
+struct SymmetricEpilogue
+{
+    Panel out, prev;
+    int64_t batch_bytes;
+    float own, before;
+    template <class T, class Acc>
+    __device__ void operator()(const T &t, Acc &acc) const
+    {
+        Panel o = out, q = prev;
+        o.base += t.z * batch_bytes;
+        if (q.base)
+            q.base += t.z * batch_bytes;
+#pragma unroll
+        for (int mi = 0; mi < T::MI; ++mi)
+#pragma unroll
+            for (int ni = 0; ni < T::NI; ++ni)
+            {
+                f32x16 &c = acc[mi][ni];
+                const int64_t rb = t.row_block(mi), cb = t.col_block(ni);
+                to_columns(c);
+                if (q.base)
+                    combine(c, q, cb, rb, t.lane, own, before);
+                else
+                {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        c[e] *= own;
+                }
+                store_columns(o, cb, rb, t.lane, c);
+                if (t.tm != t.tn)
+                    store_mirror(o, rb, cb, t.lane, c, t.wave_scratch());
+            }
+    }
+};
+
+// X <- a X + B X, as rows of n (columns of this product) and rows of m
+struct StepEpilogue
+{
+    Panel prev, columns, rows;
+    int64_t batch_bytes;
+    float own, before;
+    template <class T, class Acc>
+    __device__ void operator()(const T &t, Acc &acc) const
+    {
+        Panel q = prev, oc = columns, orow = rows;
+        q.base += t.z * batch_bytes, oc.base += t.z * batch_bytes, orow.base += t.z * batch_bytes;
+#pragma unroll
+        for (int mi = 0; mi < T::MI; ++mi)
+#pragma unroll
+            for (int ni = 0; ni < T::NI; ++ni)
+            {
+                f32x16 &c = acc[mi][ni];
+                const int64_t rb = t.row_block(mi), cb = t.col_block(ni);
+                to_columns(c);
+                combine(c, q, cb, rb, t.lane, own, before);
+                store_columns(oc, cb, rb, t.lane, c);
+                store_mirror(orow, rb, cb, t.lane, c, t.wave_scratch());
+            }
+    }
+};
+
+// the last step: X itself, or the parameter it updates
+struct LastEpilogue
+{
+    Panel prev;
+    int64_t batch_bytes;
+    float own, before;
+    Matrices a;
+    float keep, rate;  // p * keep - X * rate
+    template <class T, class Acc>
+    __device__ void operator()(const T &t, Acc &acc) const
+    {
+        Panel q = prev;
+        q.base += t.z * batch_bytes;
+        const bool tall = a.rows > a.cols;
+        const int64_t m = tall ? a.cols : a.rows, n = tall ? a.rows : a.cols;
+        const float *p = a.p[t.z];
+        float *out = a.out[t.z];
+#pragma unroll
+        for (int mi = 0; mi < T::MI; ++mi)
+#pragma unroll
+            for (int ni = 0; ni < T::NI; ++ni)
+            {
+                f32x16 &c = acc[mi][ni];
+                const int64_t rb = t.row_block(mi), cb = t.col_block(ni);
+                to_columns(c);
+                combine(c, q, cb, rb, t.lane, own, before);
+                const int64_t col = cb * 32 + (t.lane & 31);
+                if (col >= n)
+                    continue;
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                {
+                    const int64_t row = rb * 32 + 16 * (e >> 3) + 8 * (t.lane >> 5) + (e & 7);
+                    if (row < m)
+                    {
+                        const int64_t at = tall ? col * m + row : row * n + col;
+                        out[at] = p ? p[at] * keep - c[e] * rate : c[e];
+                    }
+                }
+            }
+    }
+};
+
+struct Space
+{
+    double *sums;
+    Panel xr[2], xt[2], a, b;
+    int64_t batch_bytes;
+    size_t bytes;
+};
+
+int norm_blocks(int64_t elements)
+{
+    return (int)std::min<int64_t>(256, std::max<int64_t>(1, odl::ceil_div(elements, 2048)));
+}
+
+Space space_for(char *base, int count, int64_t rows, int64_t cols)
+{
+    const int64_t mp = padded(std::min(rows, cols)), np = padded(std::max(rows, cols));
+    Space s;
+    const int64_t sums = (odl::ceil_div((int64_t)count * norm_blocks(rows * cols) * 8, 256)) * 256;
+    const int64_t xb = panel_bytes(mp, np), ab = panel_bytes(mp, mp);
+    s.batch_bytes = 4 * xb + 2 * ab;
+    char *at      = base + sums;
+    s.sums        = reinterpret_cast<double *>(base);
+    for (int i = 0; i < 2; ++i)
+        s.xr[i] = Panel{at + 2 * i * xb, np / 16}, s.xt[i] = Panel{at + (2 * i + 1) * xb, mp / 16};
+    s.a     = Panel{at + 4 * xb, mp / 16};
+    s.b     = Panel{at + 4 * xb + ab, mp / 16};
+    s.bytes = (size_t)(sums + count * s.batch_bytes);
+    return s;
+}
+
+// how many equal matrices go through the launches together: what 2 GiB of workspace holds
+int group_of(int count, int64_t rows, int64_t cols)
+{
+    const int64_t each = space_for(nullptr, 1, rows, cols).batch_bytes;
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(count, kGroup), ((int64_t)2 << 30) / each));
+}
+
+// Where f's iterates take singular values from [0, 1], and what b t + c t^2 (t = s^2) reaches on the way.
+bool coefficients_ok(double a, double b, double c, int steps)
+{
+    double top = 1.0;
+    for (int k = 0; k < steps; ++k)
+    {
+        double next = 0.0;
+        for (int i = 0; i <= 2048; ++i)
+        {
+            const double s = top * i / 2048, t = s * s, poly = b * t + c * t * t;
+            next = std::max(next, std::fabs(s * (a + poly)));
+            if (!(std::fabs(poly) < kMost && t < kMost))
+                return false;
+        }
+        if (!(next < kMost && next * next < kMost))
+            return false;
+        // f may also lift what rounding left under the last top
+        top = std::max(next, 1.0);
+    }
+    return true;
+}
+
+constexpr int64_t kMostSide = (int64_t)1 << 20;
+
+int check_common(const char *who, int64_t rows, int64_t cols, int steps, float a, float b, float c, float eps)
+{
+    ODL_REQUIRE(rows >= 0 && cols >= 0 && rows <= kMostSide && cols <= kMostSide, "%s: sides of 0 to %lld, got [%lld, %lld]", who, (long long)kMostSide,
+                (long long)rows, (long long)cols);
+    ODL_REQUIRE(steps >= 1 && steps <= 100, "%s: 1 to 100 steps, got %d", who, steps);
+    ODL_REQUIRE(eps >= 0.f, "%s: eps must not be negative, got %g", who, (double)eps);
+    ODL_REQUIRE(coefficients_ok(a, b, c, steps), "%s: coefficients (%g, %g, %g) take singular values past the range of the products' operands", who, (double)a,
+                (double)b, (double)c);
+    return ODL_OK;
+}
+
+int run_group(const Matrices &mat, int count, int steps, float a, float b, float c, float eps, float keep, float rate, char *workspace, hipStream_t st)
+{
+    const Space s = space_for(workspace, count, mat.rows, mat.cols);
+    const bool tall  = mat.rows > mat.cols;
+    const int64_t m = std::min(mat.rows, mat.cols), n = std::max(mat.rows, mat.cols), mp = padded(m), np = padded(n);
+    const int parts = norm_blocks(mat.rows * mat.cols);
+    muon_norm_kernel<<<dim3((unsigned)parts, (unsigned)count), dim3(kBlock), 0, st>>>(mat, s.sums);
+    ODL_LAUNCH_CHECK();
+    const int64_t rp = tall ? np : mp, cp = tall ? mp : np;
+    muon_prepare_kernel<<<dim3((unsigned)(cp / 64), (unsigned)(rp / 64), (unsigned)count), dim3(kBlock), 0, st>>>(
+        mat, s.sums, parts, (double)eps, tall ? s.xt[0] : s.xr[0], tall ? s.xr[0] : s.xt[0], s.batch_bytes);
+    ODL_LAUNCH_CHECK();
+    const int sym_tile = pick_tile(mp, mp, true, count), tile = pick_tile(mp, np, false, count);
+    for (int k = 0; k < steps; ++k)
+    {
+        const Panel xr = s.xr[k & 1], xt = s.xt[k & 1];
+        GemmArgs g{};
+        g.batch = count, g.a_batch = g.b_batch = s.batch_bytes;
+        g.symmetric = 1;
+        g.a = xr, g.b = xr, g.nkb = contraction_blocks(n);
+        if (int rc = launch_gemm(g, mp, mp, sym_tile, SymmetricEpilogue{s.a, Panel{nullptr, 0}, s.batch_bytes, 1.f / kScale, 0.f}, st))
+            return rc;
+        g.a = s.a, g.b = s.a, g.nkb = contraction_blocks(m);
+        if (int rc = launch_gemm(g, mp, mp, sym_tile, SymmetricEpilogue{s.b, s.a, s.batch_bytes, c / kScale, b}, st))
+            return rc;
+        g.symmetric = 0;
+        g.a = s.b, g.b = xt;
+        int rc;
+        if (k + 1 < steps)
+            rc = launch_gemm(g, mp, np, tile, StepEpilogue{xt, s.xt[(k + 1) & 1], s.xr[(k + 1) & 1], s.batch_bytes, 1.f / kScale, a}, st);
+        else
+            rc = launch_gemm(g, mp, np, tile, LastEpilogue{xt, s.batch_bytes, 1.f / kScale / kScale, a / kScale, mat, keep, rate}, st);
+        if (rc)
+            return rc;
+    }
+    return ODL_OK;
+}
+}  // namespace
+
+extern "C" size_t odl_hip_newton_schulz_workspace_bytes(int64_t batch, int64_t rows, int64_t cols)
+{
+    if (batch <= 0 || rows <= 0 || cols <= 0 || rows > kMostSide || cols > kMostSide)
+        return 0;
+    return space_for(nullptr, group_of((int)std::min<int64_t>(batch, kGroup), rows, cols), rows, cols).bytes;
+}
+
+extern "C" int odl_hip_newton_schulz(const float *g, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c, float eps, float *out,
+                                     void *workspace, size_t workspace_bytes, void *stream)
+{
+    const char *who = "newton_schulz";
+    ODL_REQUIRE(batch >= 0, "%s: negative batch", who);
+    if (int rc = check_common(who, rows, cols, steps, a, b, c, eps))
+        return rc;
+    if (batch == 0 || rows == 0 || cols == 0)
+        return ODL_OK;
+    ODL_REQUIRE(g && out, "%s: null argument", who);
+    const size_t need = odl_hip_newton_schulz_workspace_bytes(batch, rows, cols);
+    ODL_REQUIRE(workspace && workspace_bytes >= need, "%s: workspace of %zu bytes needed, got %zu", who, need, workspace ? workspace_bytes : (size_t)0);
+    ODL_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "%s: the workspace must be 16-byte aligned", who);
+    ODL_REQUIRE_DEVICE();
+    const int group = group_of((int)std::min<int64_t>(batch, kGroup), rows, cols);
+    for (int64_t first = 0; first < batch; first += group)
+    {
+        const int count = (int)std::min<int64_t>(group, batch - first);
+        Matrices mat{};
+        mat.rows = rows, mat.cols = cols;
+        for (int i = 0; i < count; ++i)
+            mat.g[i] = g + (first + i) * rows * cols, mat.out[i] = out + (first + i) * rows * cols;
+        if (int rc = run_group(mat, count, steps, a, b, c, eps, 1.f, 1.f, static_cast<char *>(workspace), odl::as_stream(stream)))
+            return rc;
+    }
+    return ODL_OK;
+}
+
+extern "C" size_t odl_hip_muon_step_multi_workspace_bytes(int count, const int64_t *host_rows, const int64_t *host_cols)
+{
+    size_t most = 0;
+    for (int i = 0; i < count && host_rows && host_cols; ++i)
+    {
+        int equal = 0;
+        for (int j = 0; j < count; ++j)
+            equal += host_rows[j] == host_rows[i] && host_cols[j] == host_cols[i];
+        most = std::max(most, odl_hip_newton_schulz_workspace_bytes(equal, host_rows[i], host_cols[i]));
+    }
+    return most;
+}
+
+extern "C" int odl_hip_muon_step_multi(int count, const float *const *p, const float *const *g, float *const *buf, const int64_t *host_rows,
+                                       const int64_t *host_cols, float lr, float momentum, int nesterov, float weight_decay, int steps, float a, float b,
+                                       float c, float eps, float *const *p_out, void *workspace, size_t workspace_bytes, void *stream)
+{
+    const char *who = "muon_step_multi";
+    ODL_REQUIRE(count >= 0, "%s: negative count", who);
+    if (count == 0)
+        return ODL_OK;
+    ODL_REQUIRE(p && g && buf && host_rows && host_cols && p_out, "%s: null argument", who);
+    for (int i = 0; i < count; ++i)
+    {
+        if (int rc = check_common(who, host_rows[i], host_cols[i], i == 0 ? steps : 1, i == 0 ? a : 1.f, i == 0 ? b : 0.f, i == 0 ? c : 0.f, eps))
+            return rc;
+        ODL_REQUIRE(host_rows[i] * host_cols[i] == 0 || (p[i] && g[i] && buf[i] && p_out[i]), "%s: null pointer for entry %d", who, i);
+    }
+    const size_t need = odl_hip_muon_step_multi_workspace_bytes(count, host_rows, host_cols);
+    ODL_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "%s: workspace of %zu bytes needed, got %zu", who, need,
+                workspace ? workspace_bytes : (size_t)0);
+    ODL_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "%s: the workspace must be 16-byte aligned", who);
+    ODL_REQUIRE_DEVICE();
+    std::vector<char> done((size_t)count, 0);
+    for (int i = 0; i < count; ++i)
+    {
+        const int64_t rows = host_rows[i], cols = host_cols[i];
+        if (done[(size_t)i] || rows == 0 || cols == 0)
+            continue;
+        // all entries of this shape, a group at a time
+        int equal = 0;
+        for (int j = i; j < count; ++j)
+            equal += host_rows[j] == rows && host_cols[j] == cols;
+        const int group = group_of(std::min(equal, kGroup), rows, cols);
+        const float rate = lr * (float)std::sqrt(std::max(1.0, (double)rows / (double)cols));
+        Matrices mat{};
+        mat.rows = rows, mat.cols = cols, mat.momentum = momentum, mat.nesterov = nesterov;
+        int in = 0;
+        for (int j = i; j < count; ++j)
+        {
+            if (host_rows[j] != rows || host_cols[j] != cols)
+                continue;
+            done[(size_t)j] = 1;
+            mat.g[in] = g[j], mat.buf[in] = buf[j], mat.p[in] = p[j], mat.out[in] = p_out[j], ++in, --equal;
+            if (in == group || equal == 0)
+            {
+                if (int rc = run_group(mat, in, steps, a, b, c, eps, 1.f - lr * weight_decay, rate, static_cast<char *>(workspace), odl::as_stream(stream)))
+                    return rc;
+                in = 0;
+            }
+        }
+    }
+    return ODL_OK;
+}

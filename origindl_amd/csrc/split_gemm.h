@@ -1,0 +1,422 @@
+// Float32 products on the float16 matrix instructions of gfx950, for the operators whose products are large and whose
+// epilogues do the rest of the operator's work (linear_ce.hip, muon.hip).
+//
+// Mathematics. A float32 operand, scaled by a power of two that brings its largest magnitude to [2^14, 2^15), is the sum of
+// two float16 numbers and an error: hi = fp16(x), lo = fp16(x - hi), |x - hi - lo| <= 2^-22 |x| (elements under 2^-18 of the
+// largest: 2^-40 of the largest instead, the spacing of float16's smallest numbers). Then
+//     a . b = ah.bh + ah.bl + al.bh     (+ al.bl <= 2^-22 |a||b|, left out)
+// with every product exact in float32 and all three summed into one float32 accumulator: the error of a float32 product's
+// own inputs and sums (measured against 64 bits: 0.3 to 1.0 times that of the float32 library product), at three float16
+// matrix instructions instead of the sixteen times slower float32 one.
+//
+// Layout ("panel"). An operand [rows, contraction] lies as blocks of 32 rows x 16 contraction values, 2 KB each: 1 KB of hi,
+// then 1 KB of lo, each in the order in which v_mfma_f32_32x32x16_f16 takes it (lane l: row l % 32, contraction values
+// 8 * (l / 32) .. + 7). Blocks of a row block are consecutive along the contraction. A load into LDS is then a straight copy
+// of 16 bytes a lane, a fragment is one ds_read_b128 without bank conflicts, and rows, columns and contraction values past
+// the matrix are zeros in memory, so the product's loop has no edges.
+//
+// The product. A workgroup holds a BM x BN tile; four stages of one contraction block each travel into LDS by direct loads
+// (no registers), queued four stages ahead; fragments of the next block are read while the present block multiplies. A
+// stage's three products use 4 fragments a pair of blocks where a plain float16 product reads 2 for one, so LDS needs only
+// half of its bandwidth.
+#pragma once
+#include <algorithm>
+#include <type_traits>
+
+#include "odl_common.h"
+
+namespace odl
+{
+namespace split
+{
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kBlockBytes = 2048;  // 32 rows x 16 contraction values, hi and lo
+constexpr int kStages     = 4;
+
+// A panel: where it lies and how many blocks a row block holds.
+struct Panel
+{
+    char *base;
+    int64_t kb;  // contraction blocks allocated per row block
+
+    __host__ __device__ int64_t row_block_bytes() const { return kb * kBlockBytes; }
+};
+
+// contraction blocks of a product
+inline int contraction_blocks(int64_t contraction)
+{
+    return (int)ceil_div(contraction, 32) * 2;
+}
+
+inline int64_t panel_bytes(int64_t rows_pad, int64_t contraction_pad)
+{
+    return rows_pad * contraction_pad * 4;
+}
+
+// Padded extent of a dimension that tiles will cover: whole tiles of the largest size that does not add more than a third.
+inline int64_t padded(int64_t n)
+{
+    const int64_t t = n > 768 ? 256 : n > 96 ? 128 : 64;
+    return ceil_div(n, t) * t;
+}
+
+__device__ inline void split_value(float y, _Float16 &hi, _Float16 &lo)
+{
+    hi = (_Float16)y;
+    lo = (_Float16)(y - (float)hi);
+}
+
+// where lane `lane` keeps its 8 values (hi; lo follows 1024 bytes later) of block (row block rb, contraction block kb)
+__device__ inline char *fragment(const Panel &p, int64_t rb, int64_t kb, int lane)
+{
+    return p.base + (rb * p.kb + kb) * kBlockBytes + lane * 16;
+}
+
+__device__ inline void store_fragment(const Panel &p, int64_t rb, int64_t kb, int lane, const float *v)
+{
+    half8 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+    {
+        _Float16 h, l;
+        split_value(v[i], h, l);
+        hi[i] = h, lo[i] = l;
+    }
+    char *at = fragment(p, rb, kb, lane);
+    *reinterpret_cast<half8 *>(at)        = hi;
+    *reinterpret_cast<half8 *>(at + 1024) = lo;
+}
+
+__device__ inline void load_fragment(const Panel &p, int64_t rb, int64_t kb, int lane, float *v)
+{
+    const char *at = fragment(p, rb, kb, lane);
+    const half8 hi = *reinterpret_cast<const half8 *>(at), lo = *reinterpret_cast<const half8 *>(at + 1024);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        v[i] = (float)hi[i] + (float)lo[i];
+}
+
+// 16 bytes a lane from a buffer into LDS: lane i's data lands at lds_byte_address + 16 * i. An instruction and not the
+// compiler's builtin, which would wait for all queued loads before every LDS read; the waits are placed by hand.
+__device__ inline void load_to_lds_16(i32x4 rsrc, unsigned lds_byte_address, unsigned lane_offset, unsigned offset)
+{
+    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :
+                 : "s"(lds_byte_address), "v"(lane_offset), "s"(rsrc), "s"(offset)
+                 : "memory", "m0");
+}
+
+__device__ inline i32x4 buffer_of(const char *base)
+{
+    const uint64_t p = reinterpret_cast<uint64_t>(base);
+    i32x4 r;
+    r[0] = __builtin_amdgcn_readfirstlane((int)(uint32_t)p);
+    r[1] = __builtin_amdgcn_readfirstlane((int)(uint32_t)(p >> 32));  // stride 0: a raw buffer
+    r[2] = 0x7fffffff;
+    r[3] = 0x00020000;
+    return r;
+}
+
+// waits until at most `vm` of the wave's vector-memory operations are outstanding and all of its LDS reads are done
+template <int vm>
+__device__ inline void wait_loads_and_lds()
+{
+    static_assert(vm >= 0 && vm < 64, "vmcnt is a 6-bit counter");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(vm) : "memory");
+}
+__device__ inline void barrier()
+{
+    asm volatile("s_barrier" ::: "memory");
+}
+
+// A 32x32 accumulator block holds, in lane l, column l % 32 and rows 8q + 4(l / 32) + r in element 4q + r. Exchanging halves of
+// the wave between neighbouring quads leaves rows 8(l / 32) + e in element e and 16 + 8(l / 32) + e in element 8 + e: eight
+// consecutive rows of one column, which is a lane's part of a fragment of the transposed block.
+__device__ inline void to_columns(f32x16 &c)
+{
+#pragma unroll
+    for (int q = 0; q < 4; q += 2)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+        {
+            const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(c[4 * q + r]), __float_as_uint(c[4 * q + 4 + r]), false, false);
+            c[4 * q + r]     = __uint_as_float(s[0]);
+            c[4 * q + 4 + r] = __uint_as_float(s[1]);
+        }
+}
+
+struct GemmArgs
+{
+    Panel a, b;       // C[i][j] = sum over the contraction of a[i][.] b[j][.]
+    int nkb;          // contraction blocks multiplied: even (panels are padded to fours, with zeros)
+    int tiles_m, tiles_n;
+    int symmetric;    // only tiles with tile row <= tile column
+    int batch;
+    int64_t a_batch, b_batch;  // bytes from one product's operands to the next one's
+    int xcds;
+    int64_t blocks() const
+    {
+        return (int64_t)batch * (symmetric ? (int64_t)tiles_m * (tiles_m + 1) / 2 : (int64_t)tiles_m * tiles_n);
+    }
+};
+
+// Which tile a workgroup computes. Workgroups are dealt to the XCDs in turn, and each XCD has an L2 of its own: the tiles are
+// cut into one run per XCD, and inside a run they go down groups of four tile rows, so that what an XCD holds at a time is a
+// compact rectangle whose operands it reads once.
+__device__ inline void tile_of(const GemmArgs &g, int &z, int &tm, int &tn)
+{
+    const unsigned total = gridDim.x, xcds = (unsigned)g.xcds, bid = blockIdx.x;
+    const unsigned x = bid % xcds, q = total / xcds, rem = total % xcds;
+    unsigned t = x * q + (x < rem ? x : rem) + bid / xcds;
+    if (g.symmetric)
+    {
+        const unsigned per = (unsigned)g.tiles_m * (g.tiles_m + 1) / 2;
+        z = (int)(t / per), t -= (unsigned)z * per;
+        int j = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+        while ((unsigned)j * (j + 1) / 2 > t)
+            --j;
+        while ((unsigned)(j + 1) * (j + 2) / 2 <= t)
+            ++j;
+        tn = j, tm = (int)(t - (unsigned)j * (j + 1) / 2);
+        return;
+    }
+    const unsigned per = (unsigned)g.tiles_m * g.tiles_n;
+    z = (int)(t / per), t -= (unsigned)z * per;
+    const unsigned gsz = 4u * g.tiles_n, grp = t / gsz, in = t - grp * gsz, first = grp * 4;
+    const unsigned rows = min(4u, (unsigned)g.tiles_m - first);
+    tm = (int)(first + in % rows), tn = (int)(in / rows);
+}
+
+// What an epilogue is handed: its accumulators stay in the kernel, one call per workgroup.
+template <int BM, int BN, int WM, int WN>
+struct Tile
+{
+    static constexpr int MI = BM / 32 / WM, NI = BN / 32 / WN;
+    static constexpr int kRows = BM, kCols = BN, kWavesM = WM, kWavesN = WN;
+    int z, tm, tn;     // product, tile row, tile column
+    int wm, wn, lane;  // wave's place in the tile
+    char *lds;         // the stages' LDS, free for the epilogue (every wave has passed a barrier)
+    __device__ int64_t row_block(int mi) const { return (int64_t)tm * (BM / 32) + wm * MI + mi; }
+    __device__ int64_t col_block(int ni) const { return (int64_t)tn * (BN / 32) + wn * NI + ni; }
+    __device__ float *wave_scratch() const  // 32 rows of 33 floats per wave
+    {
+        return reinterpret_cast<float *>(lds) + (wm * WN + wn) * (32 * 33);
+    }
+};
+
+template <int BM, int BN, int WM, int WN, class Epilogue>
+__global__ __launch_bounds__(64 * WM *WN, (BM >= 256 ? 2 : BM >= 128 ? 2 : 4)) void split_gemm_kernel(const GemmArgs g, const Epilogue epilogue)
+{
+    using T = Tile<BM, BN, WM, WN>;
+    constexpr int NW = WM * WN, MI = T::MI, NI = T::NI;
+    constexpr int kUnits = (BM + BN) / 32 * 2;  // KB of a stage: one load instruction of one wave each
+    static_assert(kUnits % NW == 0 && BM % (32 * WM) == 0 && BN % (32 * WN) == 0, "waves share a stage evenly");
+    constexpr int L = kUnits / NW;
+    constexpr int kStageBytes = kUnits * 1024;
+    static_assert(NW * 32 * 33 * 4 <= kStages * kStageBytes, "the epilogue's scratch lies in the stages");
+    __shared__ __attribute__((aligned(1024))) char lds[kStages * kStageBytes];
+
+    T t;
+    tile_of(g, t.z, t.tm, t.tn);
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    t.lane = threadIdx.x & 63, t.wm = wave / WN, t.wn = wave % WN, t.lds = lds;
+
+    // the wave's share of a stage: L half blocks, all of A or all of B
+    constexpr int kUnitsA = BM / 32 * 2;
+    static_assert(kUnitsA % L == 0, "a wave loads for one operand");
+    const bool for_a = wave * L < kUnitsA;
+    const int unit0  = for_a ? wave * L : wave * L - kUnitsA;
+    const int64_t rb_bytes = for_a ? g.a.row_block_bytes() : g.b.row_block_bytes();
+    const char *base = for_a ? g.a.base + t.z * g.a_batch + t.tm * (BM / 32) * rb_bytes : g.b.base + t.z * g.b_batch + t.tn * (BN / 32) * rb_bytes;
+    const i32x4 rsrc = buffer_of(base);
+    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    const unsigned lane_off = t.lane * 16;
+    unsigned unit_off[L];
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+        unit_off[i] = (unsigned)(((unit0 + i) >> 1) * rb_bytes) + (unsigned)((unit0 + i) & 1) * 1024;
+    // the wave's part of stage kb into its slot; past the last block the last one is loaded again (read by no product),
+    // so that the count of queued loads is the same in every round
+    auto queue = [&](int kb) {
+        const unsigned dst = lds0 + (unsigned)(kb % kStages) * kStageBytes + (unsigned)(wave * L) * 1024;
+        const unsigned at  = (unsigned)min(kb, g.nkb - 1) * kBlockBytes;
+#pragma unroll
+        for (int i = 0; i < L; ++i)
+            load_to_lds_16(rsrc, dst + i * 1024, lane_off, unit_off[i] + at);
+    };
+    // fragments: B's of a whole stage, A's one block at a time (registers: 2 x 16 + 2 x 8 beside 128 accumulators)
+    struct FragsB
+    {
+        half8 h[NI], l[NI];
+    };
+    struct FragA
+    {
+        half8 h, l;
+    };
+    auto read_b = [&](int kb, FragsB &f) {
+        const char *slot = lds + (kb % kStages) * kStageBytes + lane_off + (BM / 32 + t.wn * NI) * kBlockBytes;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+        {
+            f.h[i] = *reinterpret_cast<const half8 *>(slot + i * kBlockBytes);
+            f.l[i] = *reinterpret_cast<const half8 *>(slot + i * kBlockBytes + 1024);
+        }
+    };
+    auto read_a = [&](int kb, int i, FragA &f) {
+        const char *slot = lds + (kb % kStages) * kStageBytes + lane_off + (t.wm * MI + i) * kBlockBytes;
+        f.h = *reinterpret_cast<const half8 *>(slot);
+        f.l = *reinterpret_cast<const half8 *>(slot + 1024);
+    };
+    f32x16 acc[MI][NI];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                acc[i][j][e] = 0.f;
+    // One stage. A's next fragment is read under the products of the present one; before the last block's products comes the
+    // round's only barrier: every wave has read all of stage kb, whose slot takes stage kb + kStages, and stage kb + 1 has
+    // landed, whose first fragments are read under those products. P: which of the two A fragments the stage begins with.
+    FragA fa[2];
+    FragsB fb[2];
+    auto stage = [&](int kb, auto parity) {
+        constexpr int P = decltype(parity)::value, A0 = (P * MI) & 1;
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+        {
+            if (i + 1 < MI)
+                read_a(kb, i + 1, fa[(A0 + i + 1) & 1]);
+            else
+            {
+                wait_loads_and_lds<L *(kStages - 2)>();
+                barrier();
+                queue(kb + kStages);
+                read_b(kb + 1, fb[P ^ 1]);
+                read_a(kb + 1, 0, fa[(A0 + i + 1) & 1]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            const FragA &a = fa[(A0 + i) & 1];
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, fb[P].l[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.l, fb[P].h[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, fb[P].h[j], acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+
+    for (int s = 0; s < kStages; ++s)
+        queue(s);
+    wait_loads_and_lds<L *(kStages - 1)>();
+    barrier();
+    read_b(0, fb[0]);
+    read_a(0, 0, fa[0]);
+    for (int kb = 0; kb < g.nkb; kb += 2)
+    {
+        stage(kb, std::integral_constant<int, 0>{});
+        stage(kb + 1, std::integral_constant<int, 1>{});
+    }
+    wait_loads_and_lds<0>();  // no load is under way into LDS that the epilogue writes
+    barrier();
+    epilogue(t, acc);
+}
+
+// The tile size for a product of rows x cols (padded extents): the largest whose tiles still give the compute units work.
+// rounds * tile area / efficiency is compared; a 256-wide tile runs one workgroup per compute unit, the others two and four.
+inline int pick_tile(int64_t rows_pad, int64_t cols_pad, bool symmetric, int64_t batch)
+{
+    const int cus = device_cus();
+    int best = 64;
+    double best_cost = 0;
+    const int sizes[3] = {64, 128, 256}, resident[3] = {4, 2, 1};
+    const double eff[3] = {0.45, 0.75, 1.0};
+    for (int i = 0; i < 3; ++i)
+    {
+        const int s = sizes[i];
+        if (rows_pad % s || cols_pad % s)
+            continue;
+        const int64_t tm = rows_pad / s, tn = cols_pad / s, tiles = batch * (symmetric ? tm * (tm + 1) / 2 : tm * tn);
+        // full rounds, and the last one at what its workgroups per compute unit leave
+        const int64_t slots = (int64_t)cus * resident[i], full = tiles / slots, rest = tiles - full * slots;
+        const double last = rest == 0 ? 0.0 : (double)ceil_div(rest, cus) / resident[i];
+        // a lone workgroup on a compute unit does not fill it: it takes at least 1 / 0.6 of its share
+        const double cost = ((double)full + (last > 0 ? std::max(last, 0.6) : 0.0)) * resident[i] * s * s / eff[i];
+        if (best_cost == 0 || cost < best_cost)
+            best = s, best_cost = cost;
+    }
+    return best;
+}
+
+template <class Epilogue>
+inline int launch_gemm(GemmArgs g, int64_t rows_pad, int64_t cols_pad, int tile, const Epilogue &e, hipStream_t st)
+{
+    g.tiles_m = (int)(rows_pad / tile), g.tiles_n = (int)(cols_pad / tile), g.xcds = chip().xcds;
+    const int64_t blocks = g.blocks();
+    ODL_REQUIRE(blocks < ((int64_t)1 << 31), "product of too many tiles");
+    if (blocks == 0 || g.nkb == 0)
+        return fail(ODL_ERR_RUNTIME, "empty product");
+    if (tile == 256)
+        split_gemm_kernel<256, 256, 2, 4, Epilogue><<<dim3((unsigned)blocks), dim3(512), 0, st>>>(g, e);
+    else if (tile == 128)
+        split_gemm_kernel<128, 128, 2, 2, Epilogue><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(g, e);
+    else
+        split_gemm_kernel<64, 64, 2, 2, Epilogue><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(g, e);
+    ODL_LAUNCH_CHECK();
+    return ODL_OK;
+}
+
+// Values [rows, cols] into panels: `r` has the matrix's rows as rows, `t` its columns (either may have a null base). Src gives
+// the value at (row, col) in bounds, already scaled; a workgroup of 256 threads takes 64 x 64 values through LDS. Rows and
+// columns up to the padded extents are written as zeros.
+template <class Src>
+__device__ inline void split_tile(const Src &src, int64_t rows, int64_t cols, int64_t r0, int64_t c0, const Panel &r, const Panel &t,
+                                  float (*tile)[65])
+{
+    const int tid = threadIdx.x;
+    {
+        const int c = tid & 63;
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+        {
+            const int64_t row = r0 + (tid >> 6) + 4 * i, col = c0 + c;
+            v[i] = row < rows && col < cols ? src(row, col) : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            tile[(tid >> 6) + 4 * i][c] = v[i];
+    }
+    __syncthreads();
+    const int lane = tid & 63;
+#pragma unroll
+    for (int f = tid >> 6; f < 8; f += 4)  // fragments: 2 row blocks x 4 contraction blocks
+    {
+        const int rb = f >> 2, kb = f & 3;
+        float v[8];
+        if (r.base)
+        {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                v[e] = tile[rb * 32 + (lane & 31)][kb * 16 + (lane >> 5) * 8 + e];
+            store_fragment(r, r0 / 32 + rb, c0 / 16 + kb, lane, v);
+        }
+        if (t.base)
+        {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                v[e] = tile[kb * 16 + (lane >> 5) * 8 + e][rb * 32 + (lane & 31)];
+            store_fragment(t, c0 / 32 + rb, r0 / 16 + kb, lane, v);
+        }
+    }
+}
+}  // namespace split
+}  // namespace odl
