@@ -307,12 +307,11 @@ bool coefficients_ok(double a, double b, double c, int steps)
         for (int i = 0; i <= 2048; ++i)
         {
             const double s = top * i / 2048, t = s * s, poly = b * t + c * t * t;
-            next = std::max(next, std::fabs(s * (a + poly)));
-            if (!(std::fabs(poly) < kMost && t < kMost))
+            const double f = std::fabs(s * (a + poly));
+            if (!(f * f < kMost && std::fabs(poly) < kMost))  // (false for NaN too)
                 return false;
+            next = std::max(next, f);
         }
-        if (!(next < kMost && next * next < kMost))
-            return false;
         // f may also lift what rounding left under the last top
         top = std::max(next, 1.0);
     }

@@ -120,6 +120,18 @@ Tensor softmax_cross_entropy(const Tensor &x, const Tensor &target);
 // throws std::invalid_argument for one, as the reference's gather does; a recorded step cannot). `loss` is the tensor
 // softmax_cross_entropy returned while the step was recorded. Reads two words back from the device.
 bool softmax_cross_entropy_bad_label(const Tensor &loss);
+// softmax_cross_entropy(linear(x, weight, bias), target) for large vocabularies: the logits of x[N, K] are never stored,
+// neither here nor in backward. weight is [K, V] as nn::Linear keeps it, or [V, K] (LinearOp's layout, an embedding's) with
+// weight_out_in; bias (may be null) has V values. Rows whose target is ignore_index do not count: not in the mean, not in a
+// gradient, whatever x holds there; without a counted row the loss is 0. The probability is not offset before the logarithm.
+// A target outside [0, V) that is not ignore_index throws; while a step is being recorded it cannot, and
+// softmax_cross_entropy_bad_label on the returned loss tells after a replay.
+Tensor linear_softmax_cross_entropy(const Tensor &x, const Tensor &weight, const Tensor *bias, const Tensor &target, int64_t ignore_index = -100,
+                                    bool weight_out_in = false);
+// The matrix x — or every matrix of x[batch, rows, cols] — with its singular values brought towards 1: `steps` times
+// X <- a X + (b A + c A A) X with A = X X^T, from x / (||x|| + eps). What the Muon optimizer applies to its momentum.
+// Forward only (backward throws).
+Tensor newton_schulz(const Tensor &x, int steps = 5, float a = 3.4445f, float b = -4.7750f, float c = 2.0315f, float eps = 1e-7f);
 Tensor conv2d(const Tensor &x, const Tensor &W, const Tensor *b = nullptr, std::pair<int, int> stride = {1, 1},
               std::pair<int, int> pad = {0, 0});
 Tensor conv2d(const Tensor &x, const Tensor &W, const Tensor *b, int stride, int pad);

@@ -429,6 +429,16 @@ public:
     // (one small device-to-host copy; no upload of the loss afterwards)
     std::unique_ptr<Mat> softmax_cross_entropy_checked(const Mat &target, std::unique_ptr<Mat> *unit_grad = nullptr) const;
     std::unique_ptr<Mat> softmax_cross_entropy_backward_device(const Mat &target, const Mat &gy) const;
+    // Output layer and cross entropy in one (this = x[N, K], w[K, V] or [V, K] with w_out_in, b[V] or null): the logits are
+    // never stored. The loss is a device scalar with the words of odl_hip_linear_softmax_ce_forward behind it; row_stats
+    // receives what the backward pass needs besides. `checked` reads the out-of-range-label flag back (unless the labels'
+    // range is known on the host) and throws for one; without it the flag stays on the device (loss_bad_label_flag).
+    std::unique_ptr<Mat> linear_softmax_cross_entropy(const Mat &w, const Mat *b, const Mat &target, int64_t ignore_index, bool w_out_in,
+                                                      bool checked, std::unique_ptr<Mat> *row_stats) const;
+    // {gx, gw, gb}: an entry is null where want[i] is false; gy null: an upstream gradient of 1
+    std::vector<std::unique_ptr<Mat>> linear_softmax_cross_entropy_backward(const Mat &w, const Mat *b, const Mat &target, int64_t ignore_index,
+                                                                            bool w_out_in, const Mat &loss, const Mat &row_stats,
+                                                                            const Mat *gy, const bool want[3]) const;
     // include/origin/mat/origin/origin_mat.h:75: a dense copy with the dimensions in the order `dims`
     std::unique_ptr<Mat> permute(const std::vector<int> &dims) const;
     // a float32 tensor made by zeros / ones / full whose fill has not been queued yet: its one value, known on the host
@@ -502,6 +512,18 @@ public:
                                                              float eps, float lr, bool in_place, float weight_decay = 0.0f);
     static std::vector<std::unique_ptr<Mat>> sgd_step_multi(const std::vector<std::pair<const Mat *, const Mat *>> &param_grad,
                                                             float lr, bool in_place, float weight_decay = 0.0f);
+    // One step of the orthogonalised-momentum optimizer over a list of float32 device tensors, each seen as the matrix
+    // [dim 0, the rest]: momentum buffers in place, parameters as in adam_step_multi.
+    struct MuonItem
+    {
+        const Mat *param, *grad;
+        Mat *momentum;
+    };
+    static std::vector<std::unique_ptr<Mat>> muon_step_multi(const std::vector<MuonItem> &items, float lr, float momentum, bool nesterov,
+                                                             float weight_decay, int steps, const float coefficients[3], float eps,
+                                                             bool in_place);
+    // this matrix, or every matrix of a [batch, rows, cols] tensor, with its singular values brought towards 1
+    std::unique_ptr<Mat> newton_schulz(int steps, const float coefficients[3], float eps) const;
     // y += a*x for every (x, y) of the list
     static void axpy_multi(float a, const std::vector<std::pair<const Mat *, Mat *>> &x_y);
     static bool device_f32(const Mat &m);

@@ -274,6 +274,46 @@ public:
     void prepare_replay() override;
 };
 
+// Momentum whose direction is orthogonalised before it is applied, for a model's matrices; Adam for what is none. A matrix is
+// a parameter of two or more dimensions seen as [dim 0, the rest] with both larger than 1: a Linear's weight, a Conv2d's
+// filters, not a bias [1, out]. Per matrix: buf = momentum*buf + g; u = nesterov ? g + momentum*buf : buf;
+//   p = p*(1 - lr*weight_decay) - lr*sqrt(max(1, rows/cols)) * newton_schulz(u)
+// Matrices of equal shape go through the same launches. Settings are checked when the first step runs.
+struct MuonOptions
+{
+    float momentum = 0.95f;
+    bool nesterov = true;
+    float weight_decay = 0.0f;
+    int steps = 5;
+    float a = 3.4445f, b = -4.7750f, c = 2.0315f, eps = 1e-7f;
+    float adam_lr = 0.001f, adam_beta1 = 0.9f, adam_beta2 = 0.999f, adam_eps = 1e-8f;
+};
+
+class Muon : public Optimizer
+{
+public:
+    Muon(Module &target, float lr = 0.02f, const MuonOptions &options = MuonOptions());
+    std::unordered_map<std::string, std::any> state_dict() const override;
+    void load_state_dict(const std::unordered_map<std::string, std::any> &state_dict) override;
+    void prepare_replay() override { rest_.prepare_replay(); }
+    static bool is_matrix(const Parameter &param);
+
+protected:
+    void step_one(Parameter &param) override;
+    void step_all(std::vector<Parameter *> &params) override;
+
+private:
+    struct Rest : Adam  // the parameters that are no matrices
+    {
+        using Adam::Adam;
+        using Adam::step_all;
+    };
+    float lr_;
+    MuonOptions options_;
+    std::unordered_map<Parameter *, Tensor> momentum_buffers_;
+    Rest rest_;
+};
+
 // what WeightDecay::hook() wraps: a named type, so that Optimizer::step can recognise the hook and its rate
 struct WeightDecayHook
 {

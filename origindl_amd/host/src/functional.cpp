@@ -420,6 +420,53 @@ struct SoftmaxCrossEntropy : Operator  // src/operators/loss/softmax_cross_entro
     }
 };
 
+// The output layer and its loss as one operator: inputs x, weight, target and, with has_bias, the bias.
+struct LinearSoftmaxCrossEntropy : Operator
+{
+    int64_t ignore_index;
+    bool out_in;
+    std::shared_ptr<Mat> loss, row_stats;
+    LinearSoftmaxCrossEntropy(int64_t ignore, bool weight_out_in) : ignore_index(ignore), out_in(weight_out_in) {}
+    std::vector<Tensor> forward(const std::vector<Tensor> &xs) override
+    {
+        if (xs.size() != 3 && xs.size() != 4)
+            THROW_RUNTIME_ERROR("LinearSoftmaxCrossEntropy operator requires 3 or 4 inputs (x, weight, target, [bias]), but got {}", xs.size());
+        std::unique_ptr<Mat> stats;
+        Tensor out = wrap(omat(xs[0]).linear_softmax_cross_entropy(mat(xs[1]), xs.size() == 4 ? &mat(xs[3]) : nullptr, mat(xs[2]), ignore_index,
+                                                                   out_in, !cuda::is_capturing(), &stats));
+        loss      = out.impl_->data_;
+        row_stats = std::move(stats);
+        return {out};
+    }
+    std::vector<Tensor> backward(const std::vector<Tensor> &gys) override
+    {
+        const Mat *b       = inputs_.size() == 4 ? &mat(inputs_[3]) : nullptr;
+        const bool want[3] = {inputs_[0].requires_grad(), inputs_[1].requires_grad(), b && inputs_[3].requires_grad()};
+        // the ones backward() starts from are not written out to be read back
+        float seed     = 0.f;
+        const bool one = gys[0].elements() == 1 && omat(gys[0]).unwritten_constant(&seed) && seed == 1.0f;
+        const Tensor gy = one || gys[0].dtype() == DataType::kFloat32 ? gys[0] : gys[0].to(DataType::kFloat32);
+        auto g = omat(inputs_[0])
+                     .linear_softmax_cross_entropy_backward(mat(inputs_[1]), b, mat(inputs_[2]), ignore_index, out_in, *loss, *row_stats,
+                                                            one ? nullptr : &mat(gy), want);
+        std::vector<Tensor> out(inputs_.size());  // the target has no gradient
+        const size_t place[3] = {0, 1, 3};
+        for (int i = 0; i < 3; ++i)
+            if (want[i])
+                out[place[i]] = wrap(std::move(g[(size_t)i]));
+        return out;
+    }
+};
+
+struct NewtonSchulz : Operator  // forward only
+{
+    int steps;
+    float coefficients[3], eps;
+    NewtonSchulz(int n, float a, float b, float c, float e) : steps(n), coefficients{a, b, c}, eps(e) {}
+    std::vector<Tensor> forward(const std::vector<Tensor> &xs) override { return {wrap(omat(xs[0]).newton_schulz(steps, coefficients, eps))}; }
+    std::vector<Tensor> backward(const std::vector<Tensor> &) override { THROW_RUNTIME_ERROR("NewtonSchulz: backward is not implemented"); }
+};
+
 struct Conv2dOp : Operator  // src/operators/conv/conv2d.cpp:14-89
 {
     std::pair<int, int> stride, pad;
@@ -904,6 +951,20 @@ Tensor conv2d_relu_max_pool2d(const Tensor &x, const Tensor &W, const Tensor *b,
 Tensor softmax(const Tensor &x, int axis) { return apply<Softmax>({x}, axis); }
 Tensor softmax_cross_entropy(const Tensor &x, const Tensor &t) { return apply<SoftmaxCrossEntropy>({x, t}); }
 bool softmax_cross_entropy_bad_label(const Tensor &loss) { return SoftmaxCrossEntropy::bad_label(loss); }
+
+Tensor linear_softmax_cross_entropy(const Tensor &x, const Tensor &weight, const Tensor *bias, const Tensor &target, int64_t ignore_index,
+                                    bool weight_out_in)
+{
+    std::vector<Tensor> in{x, weight, target};
+    if (bias)
+        in.push_back(*bias);
+    return apply<LinearSoftmaxCrossEntropy>(in, ignore_index, weight_out_in);
+}
+
+Tensor newton_schulz(const Tensor &x, int steps, float a, float b, float c, float eps)
+{
+    return apply<NewtonSchulz>({x}, steps, a, b, c, eps);
+}
 
 Tensor flatten(const Tensor &x, int start_dim, int end_dim)  // src/operators/shape/flatten.cpp
 {

@@ -2249,10 +2249,129 @@ std::unique_ptr<Mat> OriginMat::permute(const std::vector<int> &dims) const
     return out;
 }
 
+namespace
+{
+constexpr size_t kLinearCeWords = 8;  // odl_hip_linear_softmax_ce_forward's: the loss, the bad-label flag, ...
+
+// the sizes of an output layer with its loss, after the checks both passes share
+void linear_ce_sizes(const OriginMat &x, const OriginMat &w, const OriginMat *b, const OriginMat &t, bool w_out_in, int64_t *N, int64_t *K,
+                     int64_t *V)
+{
+    const Shape xs = x.shape(), ws = w.shape(), ts = t.shape();
+    if (xs.size() != 2 || ws.size() != 2)
+        THROW_INVALID_ARG("linear_softmax_cross_entropy expects x (N, K) and a 2D weight, but got {} and {}", xs.to_string(), ws.to_string());
+    const size_t in = ws[w_out_in ? 1 : 0], out = ws[w_out_in ? 0 : 1];
+    if (xs[1] != in)
+        THROW_INVALID_ARG("linear_softmax_cross_entropy: x has {} features, but the weight expects {}", xs[1], in);
+    if (ts.size() != 1 || ts[0] != xs[0])
+        THROW_INVALID_ARG("linear_softmax_cross_entropy expects target to be 1D ({},), but got shape {}", xs[0], ts.to_string());
+    if (b && (b->elements() != out || b->shape().size() < 1 || b->shape()[b->shape().size() - 1] != out))
+        THROW_INVALID_ARG("linear_softmax_cross_entropy: bias of {} values expected, but got shape {}", out, b->shape().to_string());
+    if (w.device() != x.device() || t.device() != x.device() || (b && b->device() != x.device()))
+        THROW_INVALID_ARG("linear_softmax_cross_entropy: x, weight, bias and target must be on one device");
+    *N = (int64_t)xs[0], *K = (int64_t)in, *V = (int64_t)out;
+}
+}  // namespace
+
+std::unique_ptr<Mat> OriginMat::linear_softmax_cross_entropy(const Mat &w_, const Mat *b_, const Mat &target, int64_t ignore_index,
+                                                             bool w_out_in, bool checked, std::unique_ptr<Mat> *row_stats) const
+{
+    const char *who    = "linear_softmax_cross_entropy";
+    const OriginMat &x = dev_f32(*this, who), &w = dev_f32(w_, who);
+    const OriginMat *b = b_ ? &dev_f32(*b_, who) : nullptr;
+    const OriginMat &t = as_origin(target);
+    const int is64     = label_kind(t, who);
+    int64_t N, K, V, lo = 0, hi = 0;
+    linear_ce_sizes(x, w, b, t, w_out_in, &N, &K, &V);
+    const bool known = t.storage()->int_range(&lo, &hi) && ((lo >= 0 && hi < V) || (lo == ignore_index && hi == ignore_index));
+    Workspace ws(odl_hip_linear_softmax_ce_forward_workspace_bytes(N, K, V), device().index());
+    auto storage = Storage::create(kLinearCeWords * sizeof(float), DeviceType::kCUDA, device().index());
+    auto stats   = std::make_unique<OriginMat>(Shape{(size_t)N, 2}, DataType::kFloat32, device());
+    check(odl_hip_linear_softmax_ce_forward(fp(x), fp(w), w_out_in, b ? fp(*b) : nullptr, t.storage()->data(), is64, ignore_index, N, K, V,
+                                            static_cast<float *>(storage->data()), stats->data_ptr<float>(), ws.ptr(), ws.bytes, cur()));
+    auto loss = std::make_unique<OriginMat>(std::move(storage), Shape{}, DataType::kFloat32);
+    if (checked && !known && loss->loss_bad_label_flag())
+        THROW_INVALID_ARG("linear_softmax_cross_entropy: index out of range [0, {})", V);
+    *row_stats = std::move(stats);
+    return loss;
+}
+
+std::vector<std::unique_ptr<Mat>> OriginMat::linear_softmax_cross_entropy_backward(const Mat &w_, const Mat *b_, const Mat &target,
+                                                                                   int64_t ignore_index, bool w_out_in, const Mat &loss,
+                                                                                   const Mat &row_stats, const Mat *gy, const bool want[3]) const
+{
+    const char *who    = "linear_softmax_cross_entropy";
+    const OriginMat &x = dev_f32(*this, who), &w = dev_f32(w_, who);
+    const OriginMat *b = b_ ? &dev_f32(*b_, who) : nullptr;
+    const OriginMat &t = as_origin(target);
+    const int is64     = label_kind(t, who);
+    int64_t N, K, V;
+    linear_ce_sizes(x, w, b, t, w_out_in, &N, &K, &V);
+    auto gx = want[0] ? new_like(x, x.shape()) : nullptr;
+    auto gw = want[1] ? new_like(w, w.shape()) : nullptr;
+    auto gb = want[2] && b ? new_like(*b, b->shape()) : nullptr;
+    Workspace ws(odl_hip_linear_softmax_ce_backward_workspace_bytes(N, K, V), device().index());
+    check(odl_hip_linear_softmax_ce_backward(gy ? fp(dev_f32(*gy, who)) : nullptr, fp(x), fp(w), w_out_in, b ? fp(*b) : nullptr,
+                                             t.storage()->data(), is64, ignore_index, N, K, V, fp(as_origin(loss)), fp(as_origin(row_stats)),
+                                             gx ? gx->data_ptr<float>() : nullptr, gw ? gw->data_ptr<float>() : nullptr,
+                                             gb ? gb->data_ptr<float>() : nullptr, ws.ptr(), ws.bytes, cur()));
+    std::vector<std::unique_ptr<Mat>> out;
+    out.push_back(std::move(gx)), out.push_back(std::move(gw)), out.push_back(std::move(gb));
+    return out;
+}
+
+std::vector<std::unique_ptr<Mat>> OriginMat::muon_step_multi(const std::vector<MuonItem> &items, float lr, float momentum, bool nesterov,
+                                                             float weight_decay, int steps, const float coefficients[3], float eps, bool in_place)
+{
+    const char *who    = "muon_step";
+    const size_t count = items.size();
+    std::vector<const float *> p(count), g(count);
+    std::vector<float *> buf(count), out(count);
+    std::vector<int64_t> rows(count), cols(count);
+    std::vector<std::unique_ptr<Mat>> results;
+    for (size_t i = 0; i < count; ++i)
+    {
+        const OriginMat &pm = dev_f32(*items[i].param, who), &gm = dev_f32(*items[i].grad, who), &bm = dev_f32(*items[i].momentum, who);
+        if (gm.shape() != pm.shape() || bm.shape() != pm.shape() || pm.shape().size() < 2)
+            THROW_INVALID_ARG("muon_step: parameter, gradient and momentum must have one shape of two or more dimensions, but got {} {} {}",
+                              pm.shape().to_string(), gm.shape().to_string(), bm.shape().to_string());
+        p[i] = fp(pm), g[i] = fp(gm), buf[i] = const_cast<float *>(fp(bm));
+        rows[i] = (int64_t)pm.shape()[0], cols[i] = rows[i] ? (int64_t)pm.elements() / rows[i] : 0;
+        if (in_place)
+            out[i] = const_cast<float *>(p[i]);
+        else
+        {
+            auto o = new_like(pm, pm.shape());
+            out[i] = o->data_ptr<float>();
+            results.push_back(std::move(o));
+        }
+    }
+    if (count == 0)
+        return results;
+    Workspace ws(odl_hip_muon_step_multi_workspace_bytes((int)count, rows.data(), cols.data()), items[0].param->device().index());
+    check(odl_hip_muon_step_multi((int)count, p.data(), g.data(), buf.data(), rows.data(), cols.data(), lr, momentum, nesterov, weight_decay,
+                                  steps, coefficients[0], coefficients[1], coefficients[2], eps, out.data(), ws.ptr(), ws.bytes, cur()));
+    return results;
+}
+
+std::unique_ptr<Mat> OriginMat::newton_schulz(int steps, const float coefficients[3], float eps) const
+{
+    const OriginMat &g = dev_f32(*this, "newton_schulz");
+    const size_t nd    = shape_.size();
+    if (nd != 2 && nd != 3)
+        THROW_INVALID_ARG("newton_schulz expects a matrix or a batch of matrices, but got shape {}", shape_.to_string());
+    const int64_t batch = nd == 3 ? (int64_t)shape_[0] : 1, rows = (int64_t)shape_[nd - 2], cols = (int64_t)shape_[nd - 1];
+    auto out = new_like(g, shape_);
+    Workspace ws(odl_hip_newton_schulz_workspace_bytes(batch, rows, cols), device().index());
+    check(odl_hip_newton_schulz(fp(g), batch, rows, cols, steps, coefficients[0], coefficients[1], coefficients[2], eps,
+                                out->data_ptr<float>(), ws.ptr(), ws.bytes, cur()));
+    return out;
+}
+
 bool OriginMat::loss_bad_label_flag() const
 {
     if (device().type() != DeviceType::kCUDA || dtype_ != DataType::kFloat32 || elements() != 1 || !storage_ ||
-        storage_->size() != 2 * sizeof(float))
+        (storage_->size() != 2 * sizeof(float) && storage_->size() != kLinearCeWords * sizeof(float)))
         return false;
     unsigned words[2] = {0, 0};
     no_capture("device-to-host copy");

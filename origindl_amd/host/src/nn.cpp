@@ -661,6 +661,53 @@ void Adam::prepare_replay()
     replay_scales_.upload(host.data(), host.size() * sizeof(float));
 }
 
+Muon::Muon(Module &target, float lr, const MuonOptions &options)
+    : Optimizer(target), lr_(lr), options_(options), rest_(target, options.adam_lr, options.adam_beta1, options.adam_beta2, options.adam_eps)
+{}
+
+bool Muon::is_matrix(const Parameter &param)
+{
+    const Shape s = param.shape();
+    return s.size() >= 2 && s[0] > 1 && param.elements() / s[0] > 1;
+}
+
+void Muon::step_one(Parameter &param)
+{
+    std::vector<Parameter *> one{&param};
+    step_all(one);
+}
+
+void Muon::step_all(std::vector<Parameter *> &params)
+{
+    NoGradGuard guard;
+    const bool capturing = cuda::is_capturing();
+    std::vector<Parameter *> matrices, rest;
+    for (auto *p : params)
+        (is_matrix(*p) ? matrices : rest).push_back(p);
+    std::vector<OriginMat::MuonItem> items;
+    std::vector<Tensor> grads;  // keeps the gradients alive until the launches are queued
+    for (auto *p : matrices)
+    {
+        grads.push_back(p->grad());
+        const Tensor &grad = grads.back();
+        if (!momentum_buffers_.count(p))
+        {
+            if (capturing)
+                THROW_RUNTIME_ERROR("Muon: run one ordinary step before capturing (the momentum buffers must exist)");
+            momentum_buffers_.emplace(p, Tensor::zeros(grad.shape(), TensorOptions(grad.dtype()).device(grad.device())));
+        }
+        items.push_back({p->impl_->data_.get(), grad.impl_->data_.get(), momentum_buffers_.at(p).impl_->data_.get()});
+    }
+    const float coefficients[3] = {options_.a, options_.b, options_.c};
+    auto updated = OriginMat::muon_step_multi(items, lr_, options_.momentum, options_.nesterov, options_.weight_decay, options_.steps,
+                                              coefficients, options_.eps, capturing);
+    if (!capturing)
+        for (size_t i = 0; i < matrices.size(); ++i)
+            *matrices[i] = as_leaf(Tensor(std::move(updated[i])));
+    if (!rest.empty())
+        rest_.step_all(rest);
+}
+
 std::function<void(std::vector<Parameter *> &)> WeightDecay::hook() const
 {
     return WeightDecayHook{rate_};
@@ -831,6 +878,39 @@ std::unordered_map<std::string, std::any> SGD::state_dict() const
         state["momentum_buffers"] = buffers;
     }
     return state;
+}
+
+// Muon's own settings and momentum buffers, and its Adam's state under Adam's keys (its lr and eps as adam_lr, adam_eps).
+std::unordered_map<std::string, std::any> Muon::state_dict() const
+{
+    auto state = rest_.state_dict();
+    state["adam_lr"] = state["lr"], state["adam_eps"] = state["eps"];
+    state["lr"] = lr_, state["momentum"] = options_.momentum, state["nesterov"] = options_.nesterov;
+    state["weight_decay"] = options_.weight_decay, state["eps"] = options_.eps, state["steps"] = options_.steps;
+    state["a"] = options_.a, state["b"] = options_.b, state["c"] = options_.c;
+    const auto named = static_cast<const Module *>(target_)->named_parameters("");
+    StateDict buffers;
+    for (const auto &kv : momentum_buffers_)
+        if (const std::string n = name_of(named, kv.first); !n.empty())
+            buffers["momentum_" + n] = kv.second;
+    state["momentum_buffers"] = buffers;
+    return state;
+}
+
+void Muon::load_state_dict(const std::unordered_map<std::string, std::any> &sd)
+{
+    read_setting(sd, "lr", lr_), read_setting(sd, "momentum", options_.momentum), read_setting(sd, "nesterov", options_.nesterov);
+    read_setting(sd, "weight_decay", options_.weight_decay), read_setting(sd, "eps", options_.eps), read_setting(sd, "steps", options_.steps);
+    read_setting(sd, "a", options_.a), read_setting(sd, "b", options_.b), read_setting(sd, "c", options_.c);
+    auto rest = sd;
+    rest.erase("lr"), rest.erase("eps");
+    if (auto it = sd.find("adam_lr"); it != sd.end())
+        rest["lr"] = it->second;
+    if (auto it = sd.find("adam_eps"); it != sd.end())
+        rest["eps"] = it->second;
+    rest_.load_state_dict(rest);
+    auto named = target_->named_parameters("");
+    read_buffers(sd, "momentum_buffers", "momentum_", named, momentum_buffers_);
 }
 
 // The reference compares a ten-character prefix with the nine-character "momentum_" and so never restores a

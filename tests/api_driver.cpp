@@ -59,6 +59,9 @@
 #include "origin/operators/pooling/max_pool2d.h"
 #include "origin/optim/adam.h"
 #include "origin/optim/hooks.h"
+#ifdef DRV_ON_DEVICE
+#    include "origin/optim/muon.h"
+#endif
 #include "origin/optim/sgd.h"
 #include "origin/utils/metrics.h"
 
@@ -1576,6 +1579,110 @@ int DRV(mlp_bench_graph)(int64_t N, int64_t D, int64_t Hd, int64_t C, int steps,
 int DRV(cnn_bench_graph)(int64_t N, int steps, int warmup, int read_loss_each_step, float *ms_per_step, float *loss)
 {
     return cnn_bench_impl(N, steps, warmup, read_loss_each_step ? 1 : 2, ms_per_step, loss);
+}
+#endif
+
+#ifdef DRV_ON_DEVICE
+// ------------------------------------------------------------- output layer with its loss, orthogonalised updates
+// loss = cross entropy of x.w + b over the labels (nothing of size [N, V] kept); with gx: backward from loss * factor
+int DRV(linear_softmax_ce)(const float *x, const float *w, int out_in, const float *b, const void *t, int is64, int64_t ignore,
+                           int64_t N, int64_t K, int64_t V, float factor, float *loss, float *gx, float *gw, float *gb)
+{
+    return guarded([&] {
+        auto X = f32(x, Shape{(size_t)N, (size_t)K}, true);
+        auto W = f32(w, out_in ? Shape{(size_t)V, (size_t)K} : Shape{(size_t)K, (size_t)V}, true);
+        Tensor B;
+        if (b)
+            B = f32(b, Shape{1, (size_t)V}, true);
+        auto T = labels(t, is64, N);
+        auto L = F::linear_softmax_cross_entropy(X, W, b ? &B : nullptr, T, ignore, out_in != 0);
+        *loss  = L.item<float>();
+        if (!gx)
+            return;
+        if (factor == 1.0f)
+            L.backward();
+        else
+            (L * Scalar(factor)).backward();
+        out(X.grad(), gx);
+        out(W.grad(), gw);
+        if (b)
+            out(B.grad(), gb);
+    });
+}
+
+int DRV(newton_schulz)(const float *g, int64_t batch, int64_t rows, int64_t cols, int steps, float *o)
+{
+    return guarded([&] {
+        auto G = f32(g, batch > 0 ? Shape{(size_t)batch, (size_t)rows, (size_t)cols} : Shape{(size_t)rows, (size_t)cols});
+        out(F::newton_schulz(G, steps), o);
+    });
+}
+
+// MLP({D, H, V}), its last layer under linear_softmax_cross_entropy and Muon. params: w1 [D,H], b1 [H], w2 [H,V], b2 [V],
+// in and out. mode 0: plain steps; 1: the last step recorded and replayed once; 2: state_dict moved into a fresh optimizer
+// before the last step
+int DRV(muon_train)(const float *x, const int64_t *t, int64_t N, int64_t D, int64_t H, int64_t V, int steps, int mode, float lr, float decay,
+                    float adam_lr, float *params, float *losses)
+{
+    return guarded([&] {
+        nn::MLP model({(int)D, (int)H, (int)V});
+        auto &l1 = model.layer(0), &l2 = model.layer(1);
+        model.to(kDev);
+        const float *p = params;
+        auto next      = [&](Parameter *q) {
+            *q = Parameter(f32(p, q->shape(), true));
+            p += q->elements();
+        };
+        next(l1.weight()), next(l1.bias()), next(l2.weight()), next(l2.bias());
+        MuonOptions o;
+        o.weight_decay = decay, o.adam_lr = adam_lr;
+        auto opt = std::make_unique<Muon>(model, lr, o);
+        auto X = f32(x, Shape{(size_t)N, (size_t)D});
+        auto T = labels(t, 1, N);
+        auto step = [&] {
+            auto h = l1.forward_relu(X);
+            auto L = F::linear_softmax_cross_entropy(h, *l2.weight(), l2.bias(), T);
+            opt->zero_grad();
+            L.backward();
+            opt->step();
+            return L;
+        };
+        void *stream = nullptr;
+        if (mode == 1)
+            stream = origin::cuda::create_stream(), origin::cuda::set_stream(stream);
+        for (int s = 0; s < steps; ++s)
+        {
+            if (s + 1 == steps && mode == 1)
+            {
+                origin::cuda::Graph g;
+                g.begin_capture();
+                auto L = step();
+                g.end_capture();
+                opt->prepare_replay();
+                g.launch();
+                losses[s] = L.item<float>();
+                float *q = params;
+                for (auto *r : {l1.weight(), l1.bias(), l2.weight(), l2.bias()})
+                    out(*r, q), q += r->elements();
+                break;
+            }
+            if (s + 1 == steps && mode == 2)
+            {
+                auto fresh = std::make_unique<Muon>(model, 99.0f);
+                fresh->load_state_dict(opt->state_dict());
+                opt = std::move(fresh);
+            }
+            losses[s] = step().item<float>();
+        }
+        if (mode != 1)
+        {
+            float *q = params;
+            for (auto *r : {l1.weight(), l1.bias(), l2.weight(), l2.bias()})
+                out(*r, q), q += r->elements();
+        }
+        if (stream)
+            origin::cuda::set_stream(nullptr), origin::cuda::destroy_stream(stream);
+    });
 }
 #endif
 }  // extern "C"

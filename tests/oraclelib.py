@@ -122,6 +122,9 @@ _DEVICE_ONLY_SIGS = {
     "odl_host_graph_abort_recovery": "pplllpp>i",
     "odl_host_pending_fill_semantics": "lp>i",
     "odl_host_paired_layers_match_separate_modules": "lp>i",
+    "odl_host_linear_softmax_ce": "ppippillllfpppp>i",
+    "odl_host_newton_schulz": "plllip>i",
+    "odl_host_muon_train": "ppllll" "iifffpp>i",
 }
 
 
