@@ -472,6 +472,7 @@ struct OutEpilogue
 {
     float *out;
     int64_t rows, cols, ld;
+    int64_t split_stride;    // from one run of the contraction's results to the next one's
     const float *saved;
     int scale;               // kScaleX or kScaleW: whose scale the operand beside d carries
     const float *gy;
@@ -494,7 +495,7 @@ struct OutEpilogue
                     const int64_t r = t.row_block(mi) * 32 + 8 * (e >> 2) + 4 * (t.lane >> 5) + (e & 3);
                     if (r < rows)
                     {
-                        float *at = out + r * ld + col;
+                        float *at = out + t.split * split_stride + r * ld + col;
                         const float v = acc[mi][ni][e] * inv * g;
                         *at = add ? *at + v : v;
                     }
@@ -502,6 +503,18 @@ struct OutEpilogue
             }
     }
 };
+
+// gx: the runs of the contraction added up in order
+__global__ __launch_bounds__(kBlock) void ce_add_parts_kernel(const float *__restrict__ parts, int count, int64_t n, float *__restrict__ out)
+{
+    for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (int64_t)gridDim.x * kBlock)
+    {
+        float s = parts[i];
+        for (int p = 1; p < count; ++p)
+            s += parts[(int64_t)p * n + i];
+        out[i] = s;
+    }
+}
 
 // gb[v] of a piece: the partial sums of the tiles' column waves in order
 __global__ __launch_bounds__(kBlock) void ce_bias_grad_kernel(const float *__restrict__ sums, int parts, int64_t v_pad, int64_t vn, const float *saved, const float *gy,
@@ -526,6 +539,7 @@ __global__ __launch_bounds__(kBlock) void ce_bias_grad_kernel(const float *__res
 struct Plan
 {
     int64_t n_pad, k_pad, v_piece, pieces;
+    Cut gx;  // of a whole piece; its runs of the contraction add up over the pieces, each in its own place
     int64_t vn(int64_t V, int64_t p) const { return std::min(v_piece, V - p * v_piece); }
 };
 
@@ -540,6 +554,7 @@ Plan make_plan(int64_t N, int64_t K, int64_t V, bool backward)
     p.pieces  = odl::ceil_div(V, most);
     p.v_piece = p.pieces == 1 ? V : odl::ceil_div(odl::ceil_div(V, p.pieces), 256) * 256;
     p.pieces  = odl::ceil_div(V, p.v_piece);
+    p.gx      = pick_cut(p.n_pad, p.k_pad, false, 1, contraction_blocks(p.v_piece), true, (double)N * (double)K * 4 / (double)p.pieces);
     return p;
 }
 
@@ -582,7 +597,7 @@ ForwardSpace forward_space(char *base, const Plan &p, int64_t N, int64_t K, int6
     const int64_t v_pad = padded(p.v_piece);
     int64_t tiles = 0;  // of the vocabulary, over all pieces
     for (int64_t i = 0; i < p.pieces; ++i)
-        tiles += padded(p.vn(V, i)) / pick_tile(padded(p.vn(V, i)), p.n_pad, false, 1);
+        tiles += padded(p.vn(V, i)) / pick_cut(padded(p.vn(V, i)), p.n_pad, false, 1, contraction_blocks(K)).bm;
     s.mags        = c.take<float>((size_t)(magnitude_blocks(N * K) + magnitude_blocks(K * V)) * 4);
     s.bias        = c.take<float>((size_t)v_pad * 4);
     s.part_m      = c.take<float>((size_t)(tiles * p.n_pad) * 4);
@@ -598,18 +613,19 @@ ForwardSpace forward_space(char *base, const Plan &p, int64_t N, int64_t K, int6
 
 struct BackwardSpace
 {
-    float *bias, *sums;
+    float *bias, *sums, *parts;
     Panel xr, xt, wr, wt, dr, dt;
     size_t bytes;
 };
 
-BackwardSpace backward_space(char *base, const Plan &p)
+BackwardSpace backward_space(char *base, const Plan &p, int64_t N, int64_t K)
 {
     BackwardSpace s;
     Carver c{base};
     const int64_t v_pad = padded(p.v_piece);
     s.bias  = c.take<float>((size_t)v_pad * 4);
     s.sums  = c.take<float>((size_t)(p.n_pad / 32 * v_pad) * 4);
+    s.parts = c.take<float>(p.gx.splits > 1 ? (size_t)p.gx.splits * (size_t)(N * K) * 4 : 0);
     s.xr    = Panel{c.take<char>((size_t)panel_bytes(p.n_pad, p.k_pad)), p.k_pad / 16};
     s.xt    = Panel{c.take<char>((size_t)panel_bytes(p.k_pad, p.n_pad)), p.n_pad / 16};
     s.wr    = Panel{c.take<char>((size_t)panel_bytes(v_pad, p.k_pad)), p.k_pad / 16};
@@ -656,7 +672,7 @@ extern "C" size_t odl_hip_linear_softmax_ce_backward_workspace_bytes(int64_t N, 
 {
     if (N <= 0 || K <= 0 || V <= 0 || N > kMostRows || K > kMostRows || V > kMostVocabulary)
         return 0;
-    return backward_space(nullptr, make_plan(N, K, V, true)).bytes;
+    return backward_space(nullptr, make_plan(N, K, V, true), N, K).bytes;
 }
 
 extern "C" int odl_hip_linear_softmax_ce_forward(const float *x, const float *w, int w_out_in, const float *b, const void *t, int idx_is_i64,
@@ -697,11 +713,11 @@ extern "C" int odl_hip_linear_softmax_ce_forward(const float *x, const float *w,
         a.bias_blocks = (int)odl::ceil_div(v_pad, kBlock);
         ce_prepare_kernel<<<dim3((unsigned)(a.x_tiles_r * a.x_tiles_c + a.w_tiles_r * a.w_tiles_c + a.bias_blocks)), dim3(kBlock), 0, st>>>(a);
         ODL_LAUNCH_CHECK();
-        const int tile = pick_tile(v_pad, p.n_pad, false, 1);
+        const Cut cut = pick_cut(v_pad, p.n_pad, false, 1, contraction_blocks(K));
         const StatsEpilogue e{s.bias, saved8, labels, a.v0, p.n_pad, s.part_m + (int64_t)tiles_done * p.n_pad, s.part_s + (int64_t)tiles_done * p.n_pad, s.target};
-        if (int rc = launch_gemm(product(s.wr, s.xr, K), v_pad, p.n_pad, tile, e, st))
+        if (int rc = launch_gemm(product(s.wr, s.xr, K), v_pad, p.n_pad, cut, e, st))
             return rc;
-        tiles_done += (int)(v_pad / tile);
+        tiles_done += (int)(v_pad / cut.bm);
     }
     ce_join_kernel<<<dim3((unsigned)(p.n_pad / 64)), dim3(kBlock), 0, st>>>(s.part_m, s.part_s, s.target, tiles_done, p.n_pad, labels, row_stats, s.block_loss,
                                                                             s.block_count, saved8);
@@ -734,7 +750,7 @@ extern "C" int odl_hip_linear_softmax_ce_backward(const float *device_gy, const 
         return ODL_OK;
     }
     const Plan p = make_plan(N, K, V, true);
-    const BackwardSpace s = backward_space(static_cast<char *>(workspace), p);
+    const BackwardSpace s = backward_space(static_cast<char *>(workspace), p, N, K);
     ODL_REQUIRE(workspace && workspace_bytes >= s.bytes, "%s: workspace of %zu bytes needed, got %zu", who, s.bytes, workspace ? workspace_bytes : (size_t)0);
     ODL_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "%s: the workspace must be 16-byte aligned", who);
     ODL_REQUIRE_DEVICE();
@@ -754,36 +770,47 @@ extern "C" int odl_hip_linear_softmax_ce_backward(const float *device_gy, const 
         a.bias_blocks = (int)odl::ceil_div(v_pad, kBlock);
         ce_prepare_kernel<<<dim3((unsigned)(a.x_tiles_r * a.x_tiles_c + a.w_tiles_r * a.w_tiles_c + a.bias_blocks)), dim3(kBlock), 0, st>>>(a);
         ODL_LAUNCH_CHECK();
-        const int tile = pick_tile(v_pad, p.n_pad, false, 1);
+        const Cut cut = pick_cut(v_pad, p.n_pad, false, 1, contraction_blocks(K));
         GradEpilogue e{s.bias, saved8, row_stats, labels, v0, Panel{nullptr, 0}, Panel{nullptr, 0}, gb ? s.sums : nullptr, v_pad};
         if (gx)
             e.dt = s.dt;
         if (gw)
             e.dr = s.dr;
-        if (int rc = launch_gemm(product(s.wr, s.xr, K), v_pad, p.n_pad, tile, e, st))
+        if (int rc = launch_gemm(product(s.wr, s.xr, K), v_pad, p.n_pad, cut, e, st))
             return rc;
         if (gw)
         {
             // [V, K]: rows of vocabulary; [K, V]: rows of K, so that lanes run along the stored rows either way
-            const OutEpilogue o = w_out_in ? OutEpilogue{gw + v0 * K, vn, K, K, saved8, kScaleX, device_gy, 0}
-                                           : OutEpilogue{gw + v0, K, vn, V, saved8, kScaleX, device_gy, 0};
+            const OutEpilogue o = w_out_in ? OutEpilogue{gw + v0 * K, vn, K, K, 0, saved8, kScaleX, device_gy, 0}
+                                           : OutEpilogue{gw + v0, K, vn, V, 0, saved8, kScaleX, device_gy, 0};
             const int64_t rows = w_out_in ? v_pad : p.k_pad, cols = w_out_in ? p.k_pad : v_pad;
-            if (int rc = launch_gemm(w_out_in ? product(s.dr, s.xt, N) : product(s.xt, s.dr, N), rows, cols, pick_tile(rows, cols, false, 1), o, st))
+            if (int rc = launch_gemm(w_out_in ? product(s.dr, s.xt, N) : product(s.xt, s.dr, N), rows, cols, pick_cut(rows, cols, false, 1, contraction_blocks(N)), o, st))
                 return rc;
         }
         if (gx)
         {
-            const OutEpilogue o{gx, N, K, K, saved8, kScaleW, device_gy, i > 0};
-            if (int rc = launch_gemm(product(s.dt, s.wt, vn), p.n_pad, p.k_pad, pick_tile(p.n_pad, p.k_pad, false, 1), o, st))
+            // a shorter last piece keeps the runs' length: those past its end have nothing to add
+            Cut gx_cut       = p.gx;
+            const int nkb    = contraction_blocks(vn);
+            gx_cut.split_kb  = std::min(gx_cut.split_kb, nkb);
+            gx_cut.splits    = (int)odl::ceil_div(nkb, gx_cut.split_kb);
+            const OutEpilogue o{p.gx.splits > 1 ? s.parts : gx, N, K, K, N * K, saved8, kScaleW, device_gy, i > 0};
+            if (int rc = launch_gemm(product(s.dt, s.wt, vn), p.n_pad, p.k_pad, gx_cut, o, st))
                 return rc;
         }
         if (gb)
         {
-            const int waves_n = tile == 256 ? 4 : 2;
-            ce_bias_grad_kernel<<<dim3((unsigned)(v_pad / 64)), dim3(kBlock), 0, st>>>(s.sums, (int)(p.n_pad / tile) * waves_n, v_pad, vn, saved8, device_gy,
+            const int waves_n = cut.bn == 256 ? 4 : 2;
+            ce_bias_grad_kernel<<<dim3((unsigned)(v_pad / 64)), dim3(kBlock), 0, st>>>(s.sums, (int)(p.n_pad / cut.bn) * waves_n, v_pad, vn, saved8, device_gy,
                                                                                        gb + v0);
             ODL_LAUNCH_CHECK();
         }
+    }
+    if (gx && p.gx.splits > 1)
+    {
+        const int64_t n = N * K;
+        ce_add_parts_kernel<<<dim3((unsigned)std::min<int64_t>(2048, odl::ceil_div(n, kBlock))), dim3(kBlock), 0, st>>>(s.parts, p.gx.splits, n, gx);
+        ODL_LAUNCH_CHECK();
     }
     return ODL_OK;
 }

@@ -63,7 +63,24 @@ __global__ __launch_bounds__(kBlock) void muon_norm_kernel(const Matrices a, dou
     float *buf = a.buf[z];
     const Update u{a.g[z], buf, a.momentum, a.nesterov};
     double s = 0.0;
-    for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (int64_t)gridDim.x * kBlock)
+    const int64_t step = (int64_t)gridDim.x * kBlock, at = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    // four at a time where the rows of 16 bytes allow it; the rest one by one
+    const int64_t quads = ((reinterpret_cast<uintptr_t>(u.g) | reinterpret_cast<uintptr_t>(buf)) & 15) == 0 ? n / 4 : 0;
+    for (int64_t i = at; i < quads; i += step)
+    {
+        f32x4 g = reinterpret_cast<const f32x4 *>(u.g)[i];
+        if (buf)
+        {
+            f32x4 m = reinterpret_cast<f32x4 *>(buf)[i];
+            m = m * a.momentum + g;
+            reinterpret_cast<f32x4 *>(buf)[i] = m;
+            g = a.nesterov ? g + a.momentum * m : m;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            s += (double)g[e] * (double)g[e];
+    }
+    for (int64_t i = quads * 4 + at; i < n; i += step)
     {
         if (buf)
             buf[i] = buf[i] * a.momentum + u.g[i];
@@ -246,15 +263,27 @@ struct LastEpilogue
                 const int64_t col = cb * 32 + (t.lane & 31);
                 if (col >= n)
                     continue;
+                const int64_t row0 = rb * 32 + 8 * (t.lane >> 5), at0 = tall ? col * m + row0 : row0 * n + col, step = tall ? 1 : n;
+                // all of the parameter's elements are under way before the first new one is stored (p may be out)
+                float old[16];
+                if (p)
+                {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                    {
+                        const int row = 16 * (e >> 3) + (e & 7);
+                        old[e] = row0 + row < m ? p[at0 + row * step] : 0.f;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        c[e] = old[e] * keep - c[e] * rate;
+                }
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                 {
-                    const int64_t row = rb * 32 + 16 * (e >> 3) + 8 * (t.lane >> 5) + (e & 7);
-                    if (row < m)
-                    {
-                        const int64_t at = tall ? col * m + row : row * n + col;
-                        out[at] = p ? p[at] * keep - c[e] * rate : c[e];
-                    }
+                    const int row = 16 * (e >> 3) + (e & 7);
+                    if (row0 + row < m)
+                        out[at0 + row * step] = c[e];
                 }
             }
     }
@@ -270,7 +299,7 @@ struct Space
 
 int norm_blocks(int64_t elements)
 {
-    return (int)std::min<int64_t>(256, std::max<int64_t>(1, odl::ceil_div(elements, 2048)));
+    return (int)std::min<int64_t>(1024, std::max<int64_t>(1, odl::ceil_div(elements, 2048)));
 }
 
 Space space_for(char *base, int count, int64_t rows, int64_t cols)
@@ -343,26 +372,27 @@ int run_group(const Matrices &mat, int count, int steps, float a, float b, float
     muon_prepare_kernel<<<dim3((unsigned)(cp / 64), (unsigned)(rp / 64), (unsigned)count), dim3(kBlock), 0, st>>>(
         mat, s.sums, parts, (double)eps, tall ? s.xt[0] : s.xr[0], tall ? s.xr[0] : s.xt[0], s.batch_bytes);
     ODL_LAUNCH_CHECK();
-    const int sym_tile = pick_tile(mp, mp, true, count), tile = pick_tile(mp, np, false, count);
+    const int kb_m = contraction_blocks(m), kb_n = contraction_blocks(n);
+    const Cut gram = pick_cut(mp, mp, true, count, kb_n), poly = pick_cut(mp, mp, true, count, kb_m), step = pick_cut(mp, np, false, count, kb_m);
     for (int k = 0; k < steps; ++k)
     {
         const Panel xr = s.xr[k & 1], xt = s.xt[k & 1];
         GemmArgs g{};
         g.batch = count, g.a_batch = g.b_batch = s.batch_bytes;
         g.symmetric = 1;
-        g.a = xr, g.b = xr, g.nkb = contraction_blocks(n);
-        if (int rc = launch_gemm(g, mp, mp, sym_tile, SymmetricEpilogue{s.a, Panel{nullptr, 0}, s.batch_bytes, 1.f / kScale, 0.f}, st))
+        g.a = xr, g.b = xr, g.nkb = kb_n;
+        if (int rc = launch_gemm(g, mp, mp, gram, SymmetricEpilogue{s.a, Panel{nullptr, 0}, s.batch_bytes, 1.f / kScale, 0.f}, st))
             return rc;
-        g.a = s.a, g.b = s.a, g.nkb = contraction_blocks(m);
-        if (int rc = launch_gemm(g, mp, mp, sym_tile, SymmetricEpilogue{s.b, s.a, s.batch_bytes, c / kScale, b}, st))
+        g.a = s.a, g.b = s.a, g.nkb = kb_m;
+        if (int rc = launch_gemm(g, mp, mp, poly, SymmetricEpilogue{s.b, s.a, s.batch_bytes, c / kScale, b}, st))
             return rc;
         g.symmetric = 0;
         g.a = s.b, g.b = xt;
         int rc;
         if (k + 1 < steps)
-            rc = launch_gemm(g, mp, np, tile, StepEpilogue{xt, s.xt[(k + 1) & 1], s.xr[(k + 1) & 1], s.batch_bytes, 1.f / kScale, a}, st);
+            rc = launch_gemm(g, mp, np, step, StepEpilogue{xt, s.xt[(k + 1) & 1], s.xr[(k + 1) & 1], s.batch_bytes, 1.f / kScale, a}, st);
         else
-            rc = launch_gemm(g, mp, np, tile, LastEpilogue{xt, s.batch_bytes, 1.f / kScale / kScale, a / kScale, mat, keep, rate}, st);
+            rc = launch_gemm(g, mp, np, step, LastEpilogue{xt, s.batch_bytes, 1.f / kScale / kScale, a / kScale, mat, keep, rate}, st);
         if (rc)
             return rc;
     }

@@ -57,10 +57,10 @@ inline int64_t panel_bytes(int64_t rows_pad, int64_t contraction_pad)
     return rows_pad * contraction_pad * 4;
 }
 
-// Padded extent of a dimension that tiles will cover: whole tiles of the largest size that does not add more than a third.
+// Padded extent of a dimension that tiles will cover.
 inline int64_t padded(int64_t n)
 {
-    const int64_t t = n > 768 ? 256 : n > 96 ? 128 : 64;
+    const int64_t t = n > 64 ? 128 : 64;
     return ceil_div(n, t) * t;
 }
 
@@ -155,27 +155,34 @@ struct GemmArgs
     int nkb;          // contraction blocks multiplied: even (panels are padded to fours, with zeros)
     int tiles_m, tiles_n;
     int symmetric;    // only tiles with tile row <= tile column
+    int splits, split_kb;  // the contraction in `splits` runs of split_kb blocks (even), a workgroup each
     int batch;
     int64_t a_batch, b_batch;  // bytes from one product's operands to the next one's
     int xcds;
     int64_t blocks() const
     {
-        return (int64_t)batch * (symmetric ? (int64_t)tiles_m * (tiles_m + 1) / 2 : (int64_t)tiles_m * tiles_n);
+        return (int64_t)batch * splits * (symmetric ? (int64_t)tiles_m * (tiles_m + 1) / 2 : (int64_t)tiles_m * tiles_n);
     }
 };
 
 // Which tile a workgroup computes. Workgroups are dealt to the XCDs in turn, and each XCD has an L2 of its own: the tiles are
 // cut into one run per XCD, and inside a run they go down groups of four tile rows, so that what an XCD holds at a time is a
 // compact rectangle whose operands it reads once.
-__device__ inline void tile_of(const GemmArgs &g, int &z, int &tm, int &tn)
+__device__ inline void tile_of(const GemmArgs &g, int &z, int &split, int &tm, int &tn)
 {
     const unsigned total = gridDim.x, xcds = (unsigned)g.xcds, bid = blockIdx.x;
     const unsigned x = bid % xcds, q = total / xcds, rem = total % xcds;
     unsigned t = x * q + (x < rem ? x : rem) + bid / xcds;
+    const unsigned per = g.symmetric ? (unsigned)g.tiles_m * (g.tiles_m + 1) / 2 : (unsigned)g.tiles_m * g.tiles_n;
+    z = 0, split = 0;
+    if (t >= per)
+    {
+        const unsigned run = t / per;
+        t -= run * per;
+        z = (int)(run / (unsigned)g.splits), split = (int)(run - (unsigned)z * g.splits);
+    }
     if (g.symmetric)
     {
-        const unsigned per = (unsigned)g.tiles_m * (g.tiles_m + 1) / 2;
-        z = (int)(t / per), t -= (unsigned)z * per;
         int j = (int)((sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
         while ((unsigned)j * (j + 1) / 2 > t)
             --j;
@@ -184,8 +191,6 @@ __device__ inline void tile_of(const GemmArgs &g, int &z, int &tm, int &tn)
         tn = j, tm = (int)(t - (unsigned)j * (j + 1) / 2);
         return;
     }
-    const unsigned per = (unsigned)g.tiles_m * g.tiles_n;
-    z = (int)(t / per), t -= (unsigned)z * per;
     const unsigned gsz = 4u * g.tiles_n, grp = t / gsz, in = t - grp * gsz, first = grp * 4;
     const unsigned rows = min(4u, (unsigned)g.tiles_m - first);
     tm = (int)(first + in % rows), tn = (int)(in / rows);
@@ -197,7 +202,7 @@ struct Tile
 {
     static constexpr int MI = BM / 32 / WM, NI = BN / 32 / WN;
     static constexpr int kRows = BM, kCols = BN, kWavesM = WM, kWavesN = WN;
-    int z, tm, tn;     // product, tile row, tile column
+    int z, split, tm, tn;  // product, run of the contraction, tile row, tile column
     int wm, wn, lane;  // wave's place in the tile
     char *lds;         // the stages' LDS, free for the epilogue (every wave has passed a barrier)
     __device__ int64_t row_block(int mi) const { return (int64_t)tm * (BM / 32) + wm * MI + mi; }
@@ -209,7 +214,7 @@ struct Tile
 };
 
 template <int BM, int BN, int WM, int WN, class Epilogue>
-__global__ __launch_bounds__(64 * WM *WN, (BM >= 256 ? 2 : BM >= 128 ? 2 : 4)) void split_gemm_kernel(const GemmArgs g, const Epilogue epilogue)
+__global__ __launch_bounds__(64 * WM *WN, 2) void split_gemm_kernel(const GemmArgs g, const Epilogue epilogue)
 {
     using T = Tile<BM, BN, WM, WN>;
     constexpr int NW = WM * WN, MI = T::MI, NI = T::NI;
@@ -221,32 +226,36 @@ __global__ __launch_bounds__(64 * WM *WN, (BM >= 256 ? 2 : BM >= 128 ? 2 : 4)) v
     __shared__ __attribute__((aligned(1024))) char lds[kStages * kStageBytes];
 
     T t;
-    tile_of(g, t.z, t.tm, t.tn);
+    tile_of(g, t.z, t.split, t.tm, t.tn);
+    const int kb0 = t.split * g.split_kb, nkb = min(g.split_kb, g.nkb - kb0);
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     t.lane = threadIdx.x & 63, t.wm = wave / WN, t.wn = wave % WN, t.lds = lds;
 
-    // the wave's share of a stage: L half blocks, all of A or all of B
+    // the wave's share of a stage: L half blocks, A's before B's
     constexpr int kUnitsA = BM / 32 * 2;
-    static_assert(kUnitsA % L == 0, "a wave loads for one operand");
-    const bool for_a = wave * L < kUnitsA;
-    const int unit0  = for_a ? wave * L : wave * L - kUnitsA;
-    const int64_t rb_bytes = for_a ? g.a.row_block_bytes() : g.b.row_block_bytes();
-    const char *base = for_a ? g.a.base + t.z * g.a_batch + t.tm * (BM / 32) * rb_bytes : g.b.base + t.z * g.b_batch + t.tn * (BN / 32) * rb_bytes;
-    const i32x4 rsrc = buffer_of(base);
+    const char *a_base = g.a.base + t.z * g.a_batch + t.tm * (BM / 32) * g.a.row_block_bytes() + (int64_t)kb0 * kBlockBytes;
+    const char *b_base = g.b.base + t.z * g.b_batch + t.tn * (BN / 32) * g.b.row_block_bytes() + (int64_t)kb0 * kBlockBytes;
     const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
     const unsigned lane_off = t.lane * 16;
+    i32x4 rsrc[L];
     unsigned unit_off[L];
 #pragma unroll
     for (int i = 0; i < L; ++i)
-        unit_off[i] = (unsigned)(((unit0 + i) >> 1) * rb_bytes) + (unsigned)((unit0 + i) & 1) * 1024;
+    {
+        const int u = wave * L + i;
+        const bool for_a = u < kUnitsA;
+        const int v = for_a ? u : u - kUnitsA;
+        rsrc[i]     = buffer_of(for_a ? a_base : b_base);
+        unit_off[i] = (unsigned)((v >> 1) * (for_a ? g.a.row_block_bytes() : g.b.row_block_bytes())) + (unsigned)(v & 1) * 1024;
+    }
     // the wave's part of stage kb into its slot; past the last block the last one is loaded again (read by no product),
     // so that the count of queued loads is the same in every round
     auto queue = [&](int kb) {
         const unsigned dst = lds0 + (unsigned)(kb % kStages) * kStageBytes + (unsigned)(wave * L) * 1024;
-        const unsigned at  = (unsigned)min(kb, g.nkb - 1) * kBlockBytes;
+        const unsigned at  = (unsigned)min(kb, nkb - 1) * kBlockBytes;
 #pragma unroll
         for (int i = 0; i < L; ++i)
-            load_to_lds_16(rsrc, dst + i * 1024, lane_off, unit_off[i] + at);
+            load_to_lds_16(rsrc[i], dst + i * 1024, lane_off, unit_off[i] + at);
     };
     // fragments: B's of a whole stage, A's one block at a time (registers: 2 x 16 + 2 x 8 beside 128 accumulators)
     struct FragsB
@@ -320,7 +329,7 @@ __global__ __launch_bounds__(64 * WM *WN, (BM >= 256 ? 2 : BM >= 128 ? 2 : 4)) v
     barrier();
     read_b(0, fb[0]);
     read_a(0, 0, fa[0]);
-    for (int kb = 0; kb < g.nkb; kb += 2)
+    for (int kb = 0; kb < nkb; kb += 2)
     {
         stage(kb, std::integral_constant<int, 0>{});
         stage(kb + 1, std::integral_constant<int, 1>{});
@@ -330,46 +339,169 @@ __global__ __launch_bounds__(64 * WM *WN, (BM >= 256 ? 2 : BM >= 128 ? 2 : 4)) v
     epilogue(t, acc);
 }
 
-// The tile size for a product of rows x cols (padded extents): the largest whose tiles still give the compute units work.
-// rounds * tile area / efficiency is compared; a 256-wide tile runs one workgroup per compute unit, the others two and four.
-inline int pick_tile(int64_t rows_pad, int64_t cols_pad, bool symmetric, int64_t batch)
+// The product for few tiles: a workgroup of four waves holds a 64 x 64 tile, each wave the whole tile for every fourth
+// contraction block. No wave reads what another one does, so fragments come straight from memory into registers, without LDS,
+// barriers or waits for each other; the four partial sums meet in LDS at the end, added in the waves' order.
+constexpr int kDirectWaves = 4;
+
+template <class Epilogue>
+__global__ __launch_bounds__(64 * kDirectWaves, 2) void split_gemm_direct_kernel(const GemmArgs g, const Epilogue epilogue)
 {
-    const int cus = device_cus();
-    int best = 64;
-    double best_cost = 0;
-    const int sizes[3] = {64, 128, 256}, resident[3] = {4, 2, 1};
-    const double eff[3] = {0.45, 0.75, 1.0};
-    for (int i = 0; i < 3; ++i)
+    __shared__ __attribute__((aligned(16))) char lds[kDirectWaves * 4 * 4096];
+    Tile<64, 64, 2, 2> t;
+    tile_of(g, t.z, t.split, t.tm, t.tn);
+    const int kb0 = t.split * g.split_kb, nkb = min(g.split_kb, g.nkb - kb0);
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    t.lane = threadIdx.x & 63, t.lds = lds;
+    const int64_t a_rb = g.a.row_block_bytes(), b_rb = g.b.row_block_bytes();
+    const auto ra = __builtin_amdgcn_make_buffer_rsrc(g.a.base + t.z * g.a_batch + t.tm * 2 * a_rb + (int64_t)kb0 * kBlockBytes, 0, 0x7fffffff, 0x00020000);
+    const auto rb = __builtin_amdgcn_make_buffer_rsrc(g.b.base + t.z * g.b_batch + t.tn * 2 * b_rb + (int64_t)kb0 * kBlockBytes, 0, 0x7fffffff, 0x00020000);
+    struct Frags
     {
-        const int s = sizes[i];
-        if (rows_pad % s || cols_pad % s)
+        half8 ah[2], al[2], bh[2], bl[2];
+    };
+    const auto load = [&](int kb, Frags &f) {
+        // past the last block the offset lies past the buffer, and zeros arrive
+        const unsigned off = kb < nkb ? (unsigned)kb * kBlockBytes + t.lane * 16 : 0x80000000u;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+        {
+            f.ah[i] = __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(ra, off, (int)(i * a_rb), 0));
+            f.al[i] = __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(ra, off, (int)(i * a_rb) + 1024, 0));
+            f.bh[i] = __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(rb, off, (int)(i * b_rb), 0));
+            f.bl[i] = __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(rb, off, (int)(i * b_rb) + 1024, 0));
+        }
+    };
+    f32x16 acc[2][2];
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+        acc[0][0][e] = acc[0][1][e] = acc[1][0][e] = acc[1][1][e] = 0.f;
+    const auto multiply = [&](const Frags &f) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bl[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.al[i], f.bh[j], acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bh[j], acc[i][j], 0, 0, 0);
+    };
+    Frags f0, f1;
+    load(wave, f0);
+    load(wave + kDirectWaves, f1);
+    for (int kb = wave; kb < nkb; kb += 2 * kDirectWaves)
+    {
+        multiply(f0);
+        load(kb + 2 * kDirectWaves, f0);
+        multiply(f1);
+        load(kb + 3 * kDirectWaves, f1);
+    }
+    f32x4 *mine = reinterpret_cast<f32x4 *>(lds) + wave * 4 * 256 + t.lane;
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+        {
+            const f32x16 &c = acc[b >> 1][b & 1];
+            mine[b * 256 + q * 64] = f32x4{c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]};
+        }
+    __syncthreads();
+    // wave b finishes block b
+    t.wm = (wave >> 1) & 1, t.wn = wave & 1;
+    f32x16 sum[1][1];
+    {
+        const f32x4 *theirs = reinterpret_cast<const f32x4 *>(lds) + wave * 256 + t.lane;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+        {
+            f32x4 s = theirs[q * 64];
+#pragma unroll
+            for (int w = 1; w < kDirectWaves; ++w)
+                s += theirs[w * 4 * 256 + q * 64];
+            sum[0][0][4 * q] = s[0], sum[0][0][4 * q + 1] = s[1], sum[0][0][4 * q + 2] = s[2], sum[0][0][4 * q + 3] = s[3];
+        }
+    }
+    __syncthreads();  // the epilogue writes LDS
+    epilogue(t, sum);
+}
+
+// How a product is cut: tile and runs of the contraction.
+struct Cut
+{
+    int bm, bn, splits;
+    int split_kb;
+};
+
+// The cut with the least estimated time. Measured on an MI355X: microseconds per contraction block (16 values) of a tile alone
+// on its compute unit and of one among as many as fit there (256 x 256 and its halves: one; the others two), the rate in
+// TFLOP/s at which many of them run into the chip's power limit (long symmetric products lower: their tiles share less),
+// and microseconds a round of tiles spends outside its loop. Large tiles read their operands less often and leave compute
+// units idle in a short last round. Runs of the contraction (may_split) cost a pass over the partial results: out_bytes
+// written per run, read once. For example 4096 x 4096 x 4096: 323 us with 256 x 256, 325 with 256 x 128, 333 with 128 x 128, 404
+// with 64 x 64; 1024 x 1024 x 1024: 52, 29, 19 and 8.6 us.
+inline Cut pick_cut(int64_t rows_pad, int64_t cols_pad, bool symmetric, int64_t batch, int nkb, bool may_split = false, double out_bytes = 0)
+{
+    struct Option
+    {
+        int bm, bn, resident;
+        double alone, full, rate, symmetric_rate, fixed;
+    };
+    static const Option options[] = {{256, 256, 1, 0.80, 0.80, 425, 425, 12.0}, {256, 128, 1, 0.46, 0.46, 405, 405, 7.0},
+                                     {128, 256, 1, 0.46, 0.46, 405, 405, 7.0}, {128, 128, 2, 0.30, 0.26, 400, 400, 4.0},
+                                     {64, 64, 2, 0.107, 0.085, 330, 230, 2.0}};
+    const int cus = device_cus();
+    Cut best{64, 64, 1, nkb};
+    double best_cost = 0;
+    for (const Option &o : options)
+    {
+        if (rows_pad % o.bm || cols_pad % o.bn || (symmetric && o.bm != o.bn))
             continue;
-        const int64_t tm = rows_pad / s, tn = cols_pad / s, tiles = batch * (symmetric ? tm * (tm + 1) / 2 : tm * tn);
-        // full rounds, and the last one at what its workgroups per compute unit leave
-        const int64_t slots = (int64_t)cus * resident[i], full = tiles / slots, rest = tiles - full * slots;
-        const double last = rest == 0 ? 0.0 : (double)ceil_div(rest, cus) / resident[i];
-        // a lone workgroup on a compute unit does not fill it: it takes at least 1 / 0.6 of its share
-        const double cost = ((double)full + (last > 0 ? std::max(last, 0.6) : 0.0)) * resident[i] * s * s / eff[i];
-        if (best_cost == 0 || cost < best_cost)
-            best = s, best_cost = cost;
+        const int64_t tm = rows_pad / o.bm, tn = cols_pad / o.bn, tiles = batch * (symmetric ? tm * (tm + 1) / 2 : tm * tn);
+        for (int s = 1; s <= (may_split ? 32 : 1) && (s == 1 || nkb / s >= 16); ++s)
+        {
+            const int kb = s == 1 ? nkb : (int)ceil_div(nkb, 2 * s) * 2;
+            if (s > 1 && (int64_t)(s - 1) * kb >= nkb)
+                continue;
+            const int64_t work = tiles * s, slots = (int64_t)cus * o.resident, full = work / slots, rest = work - full * slots;
+            const double last = rest == 0 ? 0.0 : rest <= cus ? o.alone : o.full * (double)ceil_div(rest, cus);
+            double cost = kb * ((double)full * o.resident * o.full + last);
+            cost = std::max(cost, (double)work * kb * o.bm * o.bn * 32.0 / (symmetric ? o.symmetric_rate : o.rate) / 1e6) + o.fixed * (double)(full + (rest != 0));
+            if (s > 1)
+                cost += 3.0 + out_bytes * (s + 1) / 4e6;
+            if (best_cost == 0 || cost < best_cost)
+                best = Cut{o.bm, o.bn, s, kb}, best_cost = cost;
+        }
     }
     return best;
 }
 
 template <class Epilogue>
-inline int launch_gemm(GemmArgs g, int64_t rows_pad, int64_t cols_pad, int tile, const Epilogue &e, hipStream_t st)
+inline int launch_gemm(GemmArgs g, int64_t rows_pad, int64_t cols_pad, const Cut &cut, const Epilogue &e, hipStream_t st)
 {
-    g.tiles_m = (int)(rows_pad / tile), g.tiles_n = (int)(cols_pad / tile), g.xcds = chip().xcds;
+    g.tiles_m = (int)(rows_pad / cut.bm), g.tiles_n = (int)(cols_pad / cut.bn), g.xcds = chip().xcds;
+    g.splits = cut.splits, g.split_kb = cut.split_kb;
     const int64_t blocks = g.blocks();
     ODL_REQUIRE(blocks < ((int64_t)1 << 31), "product of too many tiles");
     if (blocks == 0 || g.nkb == 0)
         return fail(ODL_ERR_RUNTIME, "empty product");
-    if (tile == 256)
-        split_gemm_kernel<256, 256, 2, 4, Epilogue><<<dim3((unsigned)blocks), dim3(512), 0, st>>>(g, e);
-    else if (tile == 128)
-        split_gemm_kernel<128, 128, 2, 2, Epilogue><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(g, e);
+    const dim3 grid((unsigned)blocks);
+    if (cut.bm == 256 && cut.bn == 256)
+        split_gemm_kernel<256, 256, 2, 4, Epilogue><<<grid, dim3(512), 0, st>>>(g, e);
+    else if (cut.bm == 256)
+        split_gemm_kernel<256, 128, 4, 2, Epilogue><<<grid, dim3(512), 0, st>>>(g, e);
+    else if (cut.bn == 256)
+        split_gemm_kernel<128, 256, 2, 4, Epilogue><<<grid, dim3(512), 0, st>>>(g, e);
+    else if (cut.bm == 128)
+        split_gemm_kernel<128, 128, 2, 2, Epilogue><<<grid, dim3(256), 0, st>>>(g, e);
     else
-        split_gemm_kernel<64, 64, 2, 2, Epilogue><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(g, e);
+        split_gemm_direct_kernel<Epilogue><<<grid, dim3(64 * kDirectWaves), 0, st>>>(g, e);
     ODL_LAUNCH_CHECK();
     return ODL_OK;
 }
