@@ -1,0 +1,108 @@
+// What the two implementations of the output layer with its loss share: linear_ce.hip (many rows) and linear_ce_rows.hip (few).
+#pragma once
+#include <cmath>
+
+#include "odl_common.h"
+
+namespace odl
+{
+namespace linear_ce
+{
+constexpr int kBlock = 256;
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr double kLn2  = 0.69314718055994530942;
+constexpr float kDScale = 32768.f;  // d lies in [-1, 1]: two float16 numbers keep 2^-22 of an element, or 2^-40
+
+// saved[] — what the forward pass leaves for the backward pass and the caller
+enum Saved
+{
+    kLoss = 0,     // mean loss over the counted rows
+    kBadLabel,     // int: a label outside [0, V) that is not ignore_index
+    kCounted,      // rows that count
+    kScaleX,       // the powers of two the operands were multiplied by
+    kScaleW,
+    kTicket,       // int: workgroups of the joining launch that are done
+    kSavedWords = 8
+};
+
+__device__ inline int64_t label_of(const void *t, int is64, int64_t n)
+{
+    return is64 ? static_cast<const int64_t *>(t)[n] : (int64_t) static_cast<const int32_t *>(t)[n];
+}
+
+struct Labels
+{
+    const void *t;
+    int is64;
+    int64_t ignore, V, N;
+    // the row's label, or -1 where the row does not count (ignored, out of range, or past the batch)
+    __device__ int64_t operator()(int64_t n) const
+    {
+        if (n >= N)
+            return -1;
+        const int64_t l = label_of(t, is64, n);
+        return l == ignore || l < 0 || l >= V ? -1 : l;
+    }
+};
+
+// 2^v, one instruction (1 unit in the last place; results under 2^-126 are 0)
+__device__ inline float pow2(float v)
+{
+    return __builtin_amdgcn_exp2f(v);
+}
+
+// what is subtracted before 2^v: with m2 = -inf (an empty set, or logits that are all -inf) nothing, and the powers are 0
+__device__ inline float finite_top(float m2)
+{
+    return m2 == -INFINITY ? 0.f : m2;
+}
+
+// merges (m2, s) of two sets of logits. fmaxf drops NaN from the maxima, the sums keep it.
+__device__ inline void merge(float &m, float &s, float m_o, float s_o)
+{
+    const float top = fmaxf(m, m_o), sub = finite_top(top);
+    s = s * pow2(m - sub) + s_o * pow2(m_o - sub);
+    m = top;
+}
+
+
+inline size_t aligned(size_t n)
+{
+    return (n + 255) & ~(size_t)255;
+}
+
+struct Carver
+{
+    char *at;
+    size_t used = 0;
+    template <class U>
+    U *take(size_t bytes)
+    {
+        U *p = reinterpret_cast<U *>(at ? at + used : nullptr);
+        used += aligned(bytes);
+        return p;
+    }
+};
+
+
+struct Problem
+{
+    const float *x, *w, *b;
+    int w_out_in;
+    Labels labels;
+    int64_t N, K, V;
+};
+
+// Up to kFewRows rows the weights' bytes are what a pass costs, and they are read as they lie: no operand is laid out first.
+constexpr int64_t kFewRows = 64;
+size_t few_forward_bytes(int64_t N, int64_t K, int64_t V);
+size_t few_backward_bytes(int64_t N, int64_t K, int64_t V);
+int few_forward(const Problem &p, float *saved, float *row_stats, char *workspace, hipStream_t st);
+int few_backward(const Problem &p, const float *gy, const float *saved, const float *row_stats, float *gx, float *gw, float *gb, char *workspace,
+                 hipStream_t st);
+// the partial maxima and sums [tiles][n_pad] joined: row statistics, loss, flag and count; saved's ticket must be 0
+int join(const float *part_m, const float *part_s, const float *target, int64_t tiles, int64_t n_pad, const Labels &labels, float *row_stats, void *scratch,
+         float *saved, hipStream_t st);
+size_t join_scratch_bytes(int64_t N);
+}  // namespace linear_ce
+}  // namespace odl

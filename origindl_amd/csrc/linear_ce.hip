@@ -16,48 +16,13 @@
 #include <cfloat>
 #include <cmath>
 
+#include "linear_ce.h"
 #include "split_gemm.h"
 
 namespace
 {
 using namespace odl::split;
-
-constexpr int kBlock = 256;
-constexpr float kLog2e = 1.44269504088896340736f;
-constexpr double kLn2  = 0.69314718055994530942;
-constexpr float kDScale = 32768.f;  // d lies in [-1, 1]: two float16 numbers keep 2^-22 of an element, or 2^-40
-
-// saved[] — what the forward pass leaves for the backward pass and the caller
-enum Saved
-{
-    kLoss = 0,     // mean loss over the counted rows
-    kBadLabel,     // int: a label outside [0, V) that is not ignore_index
-    kCounted,      // rows that count
-    kScaleX,       // the powers of two the operands were multiplied by
-    kScaleW,
-    kTicket,       // int: workgroups of the joining launch that are done
-    kSavedWords = 8
-};
-
-__device__ inline int64_t label_of(const void *t, int is64, int64_t n)
-{
-    return is64 ? static_cast<const int64_t *>(t)[n] : (int64_t) static_cast<const int32_t *>(t)[n];
-}
-
-struct Labels
-{
-    const void *t;
-    int is64;
-    int64_t ignore, V, N;
-    // the row's label, or -1 where the row does not count (ignored, out of range, or past the batch)
-    __device__ int64_t operator()(int64_t n) const
-    {
-        if (n >= N)
-            return -1;
-        const int64_t l = label_of(t, is64, n);
-        return l == ignore || l < 0 || l >= V ? -1 : l;
-    }
-};
+using namespace odl::linear_ce;
 
 __device__ inline float block_max(float v, float *scratch)
 {
@@ -212,26 +177,6 @@ __global__ __launch_bounds__(kBlock) void ce_prepare_kernel(const PrepArgs a)
         a.bias[v] = v < a.vn ? (a.b ? a.b[a.v0 + v] : 0.f) : -INFINITY;
 }
 
-// 2^v, one instruction (1 unit in the last place; results under 2^-126 are 0)
-__device__ inline float pow2(float v)
-{
-    return __builtin_amdgcn_exp2f(v);
-}
-
-// what is subtracted before 2^v: with m2 = -inf (an empty set, or logits that are all -inf) nothing, and the powers are 0
-__device__ inline float finite_top(float m2)
-{
-    return m2 == -INFINITY ? 0.f : m2;
-}
-
-// merges (m2, s) of two sets of logits. fmaxf drops NaN from the maxima, the sums keep it.
-__device__ inline void merge(float &m, float &s, float m_o, float s_o)
-{
-    const float top = fmaxf(m, m_o), sub = finite_top(top);
-    s = s * pow2(m - sub) + s_o * pow2(m_o - sub);
-    m = top;
-}
-
 // a lane's logits of one accumulator block, rows as to_columns leaves them
 __device__ inline void logits_of(f32x16 &c, float inv_x, float inv_w, const float *bias, int lane)
 {
@@ -318,29 +263,32 @@ struct StatsEpilogue
     }
 };
 
-// Joins the partial maxima and sums of 64 tokens a workgroup; row[2n] = m2, row[2n + 1] = s; the mean loss by the last
-// workgroup to finish, which adds the workgroups' sums in their order.
+// Joins the partial maxima and sums of 16 tokens a workgroup, 16 threads a token; row[2n] = m2, row[2n + 1] = s; the mean loss
+// by the last workgroup to finish, which adds the workgroups' sums in their order.
+constexpr int kJoinRows = 16;
+
 __global__ __launch_bounds__(kBlock) void ce_join_kernel(const float *__restrict__ part_m, const float *__restrict__ part_s, const float *__restrict__ target,
-                                                         int tiles, int64_t n_pad, const Labels labels, float *__restrict__ row, double *block_loss,
+                                                         int64_t tiles, int64_t n_pad, const Labels labels, float *__restrict__ row, double *block_loss,
                                                          int *block_count, float *saved)
 {
-    __shared__ float sm[4][64], ss[4][64];
+    __shared__ float sm[16][kJoinRows], ss[16][kJoinRows];
     __shared__ int last;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t n = (int64_t)blockIdx.x * 64 + lane;
+    const int r = threadIdx.x % kJoinRows, g = threadIdx.x / kJoinRows;
+    const int64_t n = (int64_t)blockIdx.x * kJoinRows + r;
     float m = -INFINITY, s = 0.f;
-    for (int t = wave; t < tiles; t += 4)
-        merge(m, s, part_m[(int64_t)t * n_pad + n], part_s[(int64_t)t * n_pad + n]);
-    sm[wave][lane] = m, ss[wave][lane] = s;
+#pragma unroll 4
+    for (int64_t t = g; t < tiles; t += 16)
+        merge(m, s, part_m[t * n_pad + n], part_s[t * n_pad + n]);
+    sm[g][r] = m, ss[g][r] = s;
     __syncthreads();
-    if (wave == 0)
+    if (threadIdx.x < 64)
     {
-        for (int i = 1; i < 4; ++i)
-            merge(m, s, sm[i][lane], ss[i][lane]);
         double loss = 0.0;
         int count = 0, bad = 0;
-        if (n < labels.N)
+        if (threadIdx.x < kJoinRows && n < labels.N)
         {
+            for (int i = 1; i < 16; ++i)
+                merge(m, s, sm[i][r], ss[i][r]);
             row[2 * n] = m, row[2 * n + 1] = s;
             if (labels(n) >= 0)
                 loss = kLn2 * (double)m + log((double)s) - (double)target[n], count = 1;
@@ -350,7 +298,7 @@ __global__ __launch_bounds__(kBlock) void ce_join_kernel(const float *__restrict
 #pragma unroll
         for (int o = 32; o > 0; o >>= 1)
             loss += __shfl_xor(loss, o, 64), count += __shfl_xor(count, o, 64), bad |= __shfl_xor(bad, o, 64);
-        if (lane == 0)
+        if (threadIdx.x == 0)
         {
             block_loss[blockIdx.x] = loss, block_count[blockIdx.x] = bad ? ~count : count;
             __threadfence();
@@ -358,12 +306,12 @@ __global__ __launch_bounds__(kBlock) void ce_join_kernel(const float *__restrict
         }
     }
     __syncthreads();
-    if (!last || wave != 0)
+    if (!last || threadIdx.x >= 64)
         return;
     __threadfence();
     double loss = 0.0;
     int count = 0, bad = 0;
-    for (int b = lane; b < (int)gridDim.x; b += 64)
+    for (int b = threadIdx.x; b < (int)gridDim.x; b += 64)
     {
         const int c = block_count[b];
         loss += block_loss[b], count += c < 0 ? ~c : c, bad |= c < 0;
@@ -371,7 +319,7 @@ __global__ __launch_bounds__(kBlock) void ce_join_kernel(const float *__restrict
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1)
         loss += __shfl_xor(loss, o, 64), count += __shfl_xor(count, o, 64), bad |= __shfl_xor(bad, o, 64);
-    if (lane == 0)
+    if (threadIdx.x == 0)
     {
         saved[kLoss] = count ? (float)(loss / count) : 0.f;
         reinterpret_cast<int *>(saved)[kBadLabel] = bad;
@@ -558,34 +506,15 @@ Plan make_plan(int64_t N, int64_t K, int64_t V, bool backward)
     return p;
 }
 
-size_t aligned(size_t n)
-{
-    return (n + 255) & ~(size_t)255;
-}
-
 int magnitude_blocks(int64_t elements)
 {
     return (int)std::min<int64_t>(1024, std::max<int64_t>(1, odl::ceil_div(elements, 4096)));
 }
 
-struct Carver
-{
-    char *at;
-    size_t used = 0;
-    template <class U>
-    U *take(size_t bytes)
-    {
-        U *p = reinterpret_cast<U *>(at ? at + used : nullptr);
-        used += aligned(bytes);
-        return p;
-    }
-};
-
 struct ForwardSpace
 {
     float *mags, *bias, *part_m, *part_s, *target;
-    double *block_loss;
-    int *block_count;
+    void *join_scratch;
     Panel xr, wr;
     size_t bytes;
 };
@@ -603,8 +532,7 @@ ForwardSpace forward_space(char *base, const Plan &p, int64_t N, int64_t K, int6
     s.part_m      = c.take<float>((size_t)(tiles * p.n_pad) * 4);
     s.part_s      = c.take<float>((size_t)(tiles * p.n_pad) * 4);
     s.target      = c.take<float>((size_t)p.n_pad * 4);
-    s.block_loss  = c.take<double>((size_t)(p.n_pad / 64) * 8);
-    s.block_count = c.take<int>((size_t)(p.n_pad / 64) * 4);
+    s.join_scratch = c.take<void>(join_scratch_bytes(N));
     s.xr          = Panel{c.take<char>((size_t)panel_bytes(p.n_pad, p.k_pad)), p.k_pad / 16};
     s.wr          = Panel{c.take<char>((size_t)panel_bytes(v_pad, p.k_pad)), p.k_pad / 16};
     s.bytes       = c.used;
@@ -661,10 +589,34 @@ __global__ void ce_empty_kernel(float *saved)
 }
 }  // namespace
 
+namespace odl
+{
+namespace linear_ce
+{
+size_t join_scratch_bytes(int64_t N)
+{
+    return (size_t)ceil_div(N, kJoinRows) * 16;
+}
+
+int join(const float *part_m, const float *part_s, const float *target, int64_t tiles, int64_t n_pad, const Labels &labels, float *row_stats, void *scratch,
+         float *saved, hipStream_t st)
+{
+    const int64_t blocks = ceil_div(labels.N, kJoinRows);
+    double *block_loss   = static_cast<double *>(scratch);
+    ce_join_kernel<<<dim3((unsigned)blocks), dim3(kBlock), 0, st>>>(part_m, part_s, target, tiles, n_pad, labels, row_stats, block_loss,
+                                                                    reinterpret_cast<int *>(block_loss + blocks), saved);
+    ODL_LAUNCH_CHECK();
+    return ODL_OK;
+}
+}  // namespace linear_ce
+}  // namespace odl
+
 extern "C" size_t odl_hip_linear_softmax_ce_forward_workspace_bytes(int64_t N, int64_t K, int64_t V)
 {
     if (N <= 0 || K <= 0 || V <= 0 || N > kMostRows || K > kMostRows || V > kMostVocabulary)
         return 0;
+    if (N <= kFewRows)
+        return few_forward_bytes(N, K, V);
     return forward_space(nullptr, make_plan(N, K, V, false), N, K, V).bytes;
 }
 
@@ -672,6 +624,8 @@ extern "C" size_t odl_hip_linear_softmax_ce_backward_workspace_bytes(int64_t N, 
 {
     if (N <= 0 || K <= 0 || V <= 0 || N > kMostRows || K > kMostRows || V > kMostVocabulary)
         return 0;
+    if (N <= kFewRows)
+        return few_backward_bytes(N, K, V);
     return backward_space(nullptr, make_plan(N, K, V, true), N, K).bytes;
 }
 
@@ -692,16 +646,19 @@ extern "C" int odl_hip_linear_softmax_ce_forward(const float *x, const float *w,
         ODL_LAUNCH_CHECK();
         return ODL_OK;
     }
-    const Plan p = make_plan(N, K, V, false);
-    const ForwardSpace s = forward_space(static_cast<char *>(workspace), p, N, K, V);
-    ODL_REQUIRE(workspace && workspace_bytes >= s.bytes, "%s: workspace of %zu bytes needed, got %zu", who, s.bytes, workspace ? workspace_bytes : (size_t)0);
+    const size_t need = odl_hip_linear_softmax_ce_forward_workspace_bytes(N, K, V);
+    ODL_REQUIRE(workspace && workspace_bytes >= need, "%s: workspace of %zu bytes needed, got %zu", who, need, workspace ? workspace_bytes : (size_t)0);
     ODL_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "%s: the workspace must be 16-byte aligned", who);
     ODL_REQUIRE_DEVICE();
+    if (N <= kFewRows)
+        return few_forward(Problem{x, w, b, w_out_in, Labels{t, idx_is_i64, ignore_index, V, N}, N, K, V}, saved8, row_stats, static_cast<char *>(workspace), st);
+    const Plan p = make_plan(N, K, V, false);
+    const ForwardSpace s = forward_space(static_cast<char *>(workspace), p, N, K, V);
     const Labels labels{t, idx_is_i64, ignore_index, V, N};
     const int mx = magnitude_blocks(N * K), mw = magnitude_blocks(K * V);
     ce_magnitudes_kernel<<<dim3(mx + mw), dim3(kBlock), 0, st>>>(x, N, K, labels, w, K * V, mx, s.mags, saved8);
     ODL_LAUNCH_CHECK();
-    int tiles_done = 0;
+    int64_t tiles_done = 0;
     for (int64_t i = 0; i < p.pieces; ++i)
     {
         const int64_t vn = p.vn(V, i), v_pad = padded(vn);
@@ -714,15 +671,12 @@ extern "C" int odl_hip_linear_softmax_ce_forward(const float *x, const float *w,
         ce_prepare_kernel<<<dim3((unsigned)(a.x_tiles_r * a.x_tiles_c + a.w_tiles_r * a.w_tiles_c + a.bias_blocks)), dim3(kBlock), 0, st>>>(a);
         ODL_LAUNCH_CHECK();
         const Cut cut = pick_cut(v_pad, p.n_pad, false, 1, contraction_blocks(K));
-        const StatsEpilogue e{s.bias, saved8, labels, a.v0, p.n_pad, s.part_m + (int64_t)tiles_done * p.n_pad, s.part_s + (int64_t)tiles_done * p.n_pad, s.target};
+        const StatsEpilogue e{s.bias, saved8, labels, a.v0, p.n_pad, s.part_m + tiles_done * p.n_pad, s.part_s + tiles_done * p.n_pad, s.target};
         if (int rc = launch_gemm(product(s.wr, s.xr, K), v_pad, p.n_pad, cut, e, st))
             return rc;
-        tiles_done += (int)(v_pad / cut.bm);
+        tiles_done += v_pad / cut.bm;
     }
-    ce_join_kernel<<<dim3((unsigned)(p.n_pad / 64)), dim3(kBlock), 0, st>>>(s.part_m, s.part_s, s.target, tiles_done, p.n_pad, labels, row_stats, s.block_loss,
-                                                                            s.block_count, saved8);
-    ODL_LAUNCH_CHECK();
-    return ODL_OK;
+    return join(s.part_m, s.part_s, s.target, tiles_done, p.n_pad, labels, row_stats, s.join_scratch, saved8, st);
 }
 
 extern "C" int odl_hip_linear_softmax_ce_backward(const float *device_gy, const float *x, const float *w, int w_out_in, const float *b, const void *t,
@@ -749,11 +703,15 @@ extern "C" int odl_hip_linear_softmax_ce_backward(const float *device_gy, const 
                 return rc;
         return ODL_OK;
     }
-    const Plan p = make_plan(N, K, V, true);
-    const BackwardSpace s = backward_space(static_cast<char *>(workspace), p, N, K);
-    ODL_REQUIRE(workspace && workspace_bytes >= s.bytes, "%s: workspace of %zu bytes needed, got %zu", who, s.bytes, workspace ? workspace_bytes : (size_t)0);
+    const size_t need = odl_hip_linear_softmax_ce_backward_workspace_bytes(N, K, V);
+    ODL_REQUIRE(workspace && workspace_bytes >= need, "%s: workspace of %zu bytes needed, got %zu", who, need, workspace ? workspace_bytes : (size_t)0);
     ODL_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "%s: the workspace must be 16-byte aligned", who);
     ODL_REQUIRE_DEVICE();
+    if (N <= kFewRows)
+        return few_backward(Problem{x, w, b, w_out_in, Labels{t, idx_is_i64, ignore_index, V, N}, N, K, V}, device_gy, saved8, row_stats, gx, gw, gb,
+                            static_cast<char *>(workspace), st);
+    const Plan p = make_plan(N, K, V, true);
+    const BackwardSpace s = backward_space(static_cast<char *>(workspace), p, N, K);
     const Labels labels{t, idx_is_i64, ignore_index, V, N};
     for (int64_t i = 0; i < p.pieces; ++i)
     {

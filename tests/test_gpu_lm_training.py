@@ -89,7 +89,7 @@ def check(got, want, bars):
 
 # one token to many, one feature, one class, sizes around every tile (64, 128, 256) and its half, and several pieces
 CE_SHAPES = [(1, 1, 1), (1, 64, 1000), (2, 3, 5), (3, 17, 64), (5, 33, 65), (16, 100, 130), (31, 257, 511), (64, 128, 256), (65, 96, 97),
-             (96, 769, 300), (128, 64, 1025), (200, 768, 2000), (257, 130, 769), (770, 100, 3001), (1025, 300, 1100)]
+             (96, 769, 300), (128, 64, 1025), (200, 768, 2000), (257, 130, 769), (770, 100, 3001), (1025, 300, 1100), (33, 40, 129), (64, 1030, 2050), (1, 4097, 3), (8, 5, 6000), (32, 2048, 4000)]
 
 
 @pytest.mark.parametrize("shape", CE_SHAPES)
