@@ -93,8 +93,14 @@ struct Problem
     int64_t N, K, V;
 };
 
-// Up to kFewRows rows the weights' bytes are what a pass costs, and they are read as they lie: no operand is laid out first.
-constexpr int64_t kFewRows = 64;
+// Up to 64 rows the bytes of large weights are what a pass costs, and they are read as they lie: no operand is laid out first.
+// Measured with one row over 2048 x 32000: forward 78 us against 306; with 64 rows over 256 x 1000, forward and backward, the
+// operands laid out win, 68 us against 98: their launches fill the chip where the streams' tiles of 128 entries do not. The
+// estimates of both cross at about 6 million weights.
+inline bool few_rows(int64_t N, int64_t K, int64_t V)
+{
+    return N <= 64 && K * V >= 6000000;
+}
 size_t few_forward_bytes(int64_t N, int64_t K, int64_t V);
 size_t few_backward_bytes(int64_t N, int64_t K, int64_t V);
 int few_forward(const Problem &p, float *saved, float *row_stats, char *workspace, hipStream_t st);

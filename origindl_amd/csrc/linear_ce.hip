@@ -615,7 +615,7 @@ extern "C" size_t odl_hip_linear_softmax_ce_forward_workspace_bytes(int64_t N, i
 {
     if (N <= 0 || K <= 0 || V <= 0 || N > kMostRows || K > kMostRows || V > kMostVocabulary)
         return 0;
-    if (N <= kFewRows)
+    if (few_rows(N, K, V))
         return few_forward_bytes(N, K, V);
     return forward_space(nullptr, make_plan(N, K, V, false), N, K, V).bytes;
 }
@@ -624,7 +624,7 @@ extern "C" size_t odl_hip_linear_softmax_ce_backward_workspace_bytes(int64_t N, 
 {
     if (N <= 0 || K <= 0 || V <= 0 || N > kMostRows || K > kMostRows || V > kMostVocabulary)
         return 0;
-    if (N <= kFewRows)
+    if (few_rows(N, K, V))
         return few_backward_bytes(N, K, V);
     return backward_space(nullptr, make_plan(N, K, V, true), N, K).bytes;
 }
@@ -650,7 +650,7 @@ extern "C" int odl_hip_linear_softmax_ce_forward(const float *x, const float *w,
     ODL_REQUIRE(workspace && workspace_bytes >= need, "%s: workspace of %zu bytes needed, got %zu", who, need, workspace ? workspace_bytes : (size_t)0);
     ODL_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "%s: the workspace must be 16-byte aligned", who);
     ODL_REQUIRE_DEVICE();
-    if (N <= kFewRows)
+    if (few_rows(N, K, V))
         return few_forward(Problem{x, w, b, w_out_in, Labels{t, idx_is_i64, ignore_index, V, N}, N, K, V}, saved8, row_stats, static_cast<char *>(workspace), st);
     const Plan p = make_plan(N, K, V, false);
     const ForwardSpace s = forward_space(static_cast<char *>(workspace), p, N, K, V);
@@ -707,7 +707,7 @@ extern "C" int odl_hip_linear_softmax_ce_backward(const float *device_gy, const 
     ODL_REQUIRE(workspace && workspace_bytes >= need, "%s: workspace of %zu bytes needed, got %zu", who, need, workspace ? workspace_bytes : (size_t)0);
     ODL_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "%s: the workspace must be 16-byte aligned", who);
     ODL_REQUIRE_DEVICE();
-    if (N <= kFewRows)
+    if (few_rows(N, K, V))
         return few_backward(Problem{x, w, b, w_out_in, Labels{t, idx_is_i64, ignore_index, V, N}, N, K, V}, device_gy, saved8, row_stats, gx, gw, gb,
                             static_cast<char *>(workspace), st);
     const Plan p = make_plan(N, K, V, true);

@@ -78,18 +78,26 @@ __global__ __launch_bounds__(64 * kWaves, 2) void ce_stream_kernel(const Stream 
         f32x4 w[4], q[NB];
     };
     const f32x4 *q = a.q + (int64_t)half * NB * 32 + col;
-    const auto load = [&](int64_t g, Step &s) {
+    const int64_t first = ((int64_t)blockIdx.y * kWaves + wave) * a.wave_groups, last = min(first + a.wave_groups, a.groups);
+    const int64_t whole = a.outs >= 4 || OUT_ROWS ? min(last, a.contraction / 8) : first;
+    // In the last tile a lane past the outputs reads what lies in reach instead (its outputs are nobody's); of four outputs that
+    // straddle the end it reads the last four and moves them to their places.
+    const int64_t o_lane = o0 + col * 4, shift = OUT_ROWS ? 0 : o_lane + 4 - a.outs;
+    const float *w[4];
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-            s.q[nb] = q[g * 2 * NB * 32 + nb * 32];
+    for (int i = 0; i < 4; ++i)
+        w[i] = OUT_ROWS ? a.w + min(o0 + 32 * i + col, a.outs - 1) * a.ld + half * 4 : a.w + (int64_t)(half * 4 + i) * a.ld + (shift > 0 ? a.outs - 4 : o_lane);
+    const int64_t w_step = OUT_ROWS ? 8 : 8 * a.ld;
+    const auto load = [&](int64_t g, Step &s) {
+        const int64_t at = min(g, whole - 1);  // past the wave's last whole step: that one again, multiplied by nobody
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if constexpr (OUT_ROWS)
-                s.w[i] = *reinterpret_cast<const f32x4u *>(a.w + (o0 + 32 * i + col) * a.ld + g * 8 + half * 4);
-            else
-                s.w[i] = *reinterpret_cast<const f32x4u *>(a.w + (g * 8 + half * 4 + i) * a.ld + o0 + col * 4);
+            s.w[i] = *reinterpret_cast<const f32x4u *>(w[i] + at * w_step);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+            s.q[nb] = q[at * 2 * NB * 32 + nb * 32];
     };
-    // at the ends of w: single loads, zeros past them
+    // the contraction's last values, single loads with zeros past its end (and outputs fewer than four)
     const auto load_guarded = [&](int64_t g, Step &s) {
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
@@ -103,43 +111,47 @@ __global__ __launch_bounds__(64 * kWaves, 2) void ce_stream_kernel(const Stream 
                 s.w[i][e] = o < a.outs && c < a.contraction ? a.w[OUT_ROWS ? o * a.ld + c : c * a.ld + o] : 0.f;
             }
     };
-    const auto multiply = [&](const Step &s) {
+    const bool straddles = !OUT_ROWS && o0 + kTile > a.outs;
+    const auto multiply = [&](const Step &s, bool move) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
+        {
+            f32x4 v = s.w[j];
+            if (move)
+            {
+                v = shift == 1 ? f32x4{v[1], v[2], v[3], 0.f} : v;
+                v = shift == 2 ? f32x4{v[2], v[3], 0.f, 0.f} : v;
+                v = shift == 3 ? f32x4{v[3], 0.f, 0.f, 0.f} : v;
+            }
 #pragma unroll
             for (int m = 0; m < 4; ++m)
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
-                    acc[m][nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(OUT_ROWS ? s.w[m][j] : s.w[j][m], s.q[nb][j], acc[m][nb], 0, 0, 0);
+                    acc[m][nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(OUT_ROWS ? s.w[m][j] : v[m], s.q[nb][j], acc[m][nb], 0, 0, 0);
+        }
     };
-    const int64_t first = ((int64_t)blockIdx.y * kWaves + wave) * a.wave_groups, last = min(first + a.wave_groups, a.groups);
-    const int64_t whole = o0 + kTile <= a.outs ? min(last, a.contraction / 8) : first;
-    int64_t g = first;
-    if (g + 1 < whole)
+    if (first < whole)
     {
         Step s0, s1, t0, t1;
-        load(g, s0), load(g + 1, s1);
-        for (; g + 5 < whole; g += 4)
+        load(first, s0), load(first + 1, s1);
+        for (int64_t g = first; g < whole; g += 4)
         {
             load(g + 2, t0), load(g + 3, t1);
-            multiply(s0), multiply(s1);
+            multiply(s0, straddles);
+            if (g + 1 < whole)
+                multiply(s1, straddles);
             load(g + 4, s0), load(g + 5, s1);
-            multiply(t0), multiply(t1);
+            if (g + 2 < whole)
+                multiply(t0, straddles);
+            if (g + 3 < whole)
+                multiply(t1, straddles);
         }
-        multiply(s0), multiply(s1);
-        g += 2;
     }
-    for (; g < whole; ++g)
-    {
-        Step s;
-        load(g, s);
-        multiply(s);
-    }
-    for (; g < last; ++g)
+    for (int64_t g = max(first, whole); g < last; ++g)
     {
         Step s;
         load_guarded(g, s);
-        multiply(s);
+        multiply(s, false);
     }
     // the waves' sums, one block of columns at a time; wave m < 4 adds up block m in the waves' order
     f32x16 sum[NB];
@@ -328,6 +340,7 @@ __global__ __launch_bounds__(kBlock) void ce_rows_gx_kernel(const float *__restr
         const int k = i / rows, n = i % rows;
         float s = 0.f;
         if (k0 + k < K)
+#pragma unroll 8
             for (int r = 0; r < runs; ++r)
                 s += parts[((int64_t)r * K + k0 + k) * rows + n];
         tile[k][n] = s * g;
@@ -411,7 +424,7 @@ int64_t quads_of(int64_t n)
 int runs_for_gx(int64_t K, int64_t V)
 {
     const int64_t tiles = odl::ceil_div(K, kTile);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(odl::device_cus() / tiles, odl::ceil_div(V, 512)));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(odl::device_cus() / tiles, odl::ceil_div(V, 128)));
 }
 
 struct FewSpace
