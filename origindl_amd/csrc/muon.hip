@@ -16,42 +16,12 @@
 #include <cmath>
 #include <vector>
 
-#include "split_gemm.h"
+#include "muon.h"
 
 namespace
 {
 using namespace odl::split;
-
-constexpr int kBlock     = 256;
-constexpr float kScale   = 8192.f;
-constexpr double kMost   = 7.5;
-constexpr int kGroup     = 32;  // matrices per launch
-
-struct Matrices  // one launch's matrices: all [rows, cols]
-{
-    const float *g[kGroup];
-    float *buf[kGroup];    // null: U is the gradient itself
-    const float *p[kGroup];
-    float *out[kGroup];    // X, or the new parameter where p is not null
-    int64_t rows, cols;
-    float momentum;
-    int nesterov;
-
-};
-
-// U's element i; buf holds the new momentum already
-struct Update
-{
-    const float *g, *buf;
-    float momentum;
-    int nesterov;
-    __device__ float operator()(int64_t i) const
-    {
-        if (!buf)
-            return g[i];
-        return nesterov ? g[i] + momentum * buf[i] : buf[i];
-    }
-};
+using namespace odl::muon;
 
 // buf <- mu buf + g, and the partial sums of U's squares, in 64 bits: the norm's error is common to all of X, and the steps
 // amplify it
@@ -97,14 +67,6 @@ __global__ __launch_bounds__(kBlock) void muon_norm_kernel(const Matrices a, dou
         sums[(int64_t)z * gridDim.x + blockIdx.x] = (part[0] + part[1]) + (part[2] + part[3]);
 }
 
-struct ScaledUpdate
-{
-    Update u;
-    int64_t cols;
-    double factor;
-    __device__ float operator()(int64_t r, int64_t c) const { return (float)((double)u(r * cols + c) * factor); }
-};
-
 // X0 as panels: r has the matrix's rows as rows, t its columns
 __global__ __launch_bounds__(kBlock) void muon_prepare_kernel(const Matrices a, const double *sums, int parts, double eps, Panel r, Panel t,
                                                               int64_t batch_bytes)
@@ -112,64 +74,9 @@ __global__ __launch_bounds__(kBlock) void muon_prepare_kernel(const Matrices a, 
     __shared__ float tile[64][65];
     __shared__ double part[4];
     const int z = blockIdx.z;
-    double s = 0.0;
-    for (int i = threadIdx.x; i < parts; i += kBlock)
-        s += sums[(int64_t)z * parts + i];
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1)
-        s += __shfl_xor(s, o, 64);
-    if ((threadIdx.x & 63) == 0)
-        part[threadIdx.x >> 6] = s;
-    __syncthreads();
-    s = (part[0] + part[1]) + (part[2] + part[3]);
+    const double norm = sqrt(sum_of_parts<4>(sums + (int64_t)z * parts, parts, part));
     r.base += z * batch_bytes, t.base += z * batch_bytes;
-    split_tile(ScaledUpdate{{a.g[z], a.buf[z], a.momentum, a.nesterov}, a.cols, (double)kScale / (sqrt(s) + eps)}, a.rows, a.cols, (int64_t)blockIdx.y * 64, (int64_t)blockIdx.x * 64, r, t, tile);
-}
-
-// the accumulator block as rows of the other side: through the wave's scratch
-__device__ inline void store_mirror(const Panel &p, int64_t rb, int64_t cb, int lane, const f32x16 &c, float *scratch)
-{
-#pragma unroll
-    for (int e = 0; e < 16; ++e)
-        scratch[(16 * (e >> 3) + 8 * (lane >> 5) + (e & 7)) * 33 + (lane & 31)] = c[e];
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-    {
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            v[e] = scratch[(lane & 31) * 33 + 16 * h + 8 * (lane >> 5) + e];
-        store_fragment(p, rb, cb * 2 + h, lane, v);
-    }
-    __builtin_amdgcn_wave_barrier();
-}
-
-// c[8h + e] <- own * acc + before * prev at the block's place in a panel of the column side, kept times kScale
-__device__ inline void combine(f32x16 &c, const Panel &prev, int64_t cb, int64_t rb, int lane, float own, float before)
-{
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-    {
-        float v[8];
-        load_fragment(prev, cb, rb * 2 + h, lane, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            c[8 * h + e] = fmaf(own, c[8 * h + e], before * v[e]);
-    }
-}
-
-__device__ inline void store_columns(const Panel &p, int64_t cb, int64_t rb, int lane, const f32x16 &c)
-{
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-    {
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            v[e] = c[8 * h + e];
-        store_fragment(p, cb, rb * 2 + h, lane, v);
-    }
+    split_tile(ScaledUpdate{{a.g[z], a.buf[z], a.momentum, a.nesterov}, a.cols, (double)kScale / (norm + eps)}, a.rows, a.cols, (int64_t)blockIdx.y * 64, (int64_t)blockIdx.x * 64, r, t, tile);
 }
 
 // A = X X^T (prev null), or b A + c A A: symmetric, computed for tile row <= tile column
@@ -247,10 +154,6 @@ struct LastEpilogue
     {
         Panel q = prev;
         q.base += t.z * batch_bytes;
-        const bool tall = a.rows > a.cols;
-        const int64_t m = tall ? a.cols : a.rows, n = tall ? a.rows : a.cols;
-        const float *p = a.p[t.z];
-        float *out = a.out[t.z];
 #pragma unroll
         for (int mi = 0; mi < T::MI; ++mi)
 #pragma unroll
@@ -260,31 +163,7 @@ struct LastEpilogue
                 const int64_t rb = t.row_block(mi), cb = t.col_block(ni);
                 to_columns(c);
                 combine(c, q, cb, rb, t.lane, own, before);
-                const int64_t col = cb * 32 + (t.lane & 31);
-                if (col >= n)
-                    continue;
-                const int64_t row0 = rb * 32 + 8 * (t.lane >> 5), at0 = tall ? col * m + row0 : row0 * n + col, step = tall ? 1 : n;
-                // all of the parameter's elements are under way before the first new one is stored (p may be out)
-                float old[16];
-                if (p)
-                {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                    {
-                        const int row = 16 * (e >> 3) + (e & 7);
-                        old[e] = row0 + row < m ? p[at0 + row * step] : 0.f;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        c[e] = old[e] * keep - c[e] * rate;
-                }
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                {
-                    const int row = 16 * (e >> 3) + (e & 7);
-                    if (row0 + row < m)
-                        out[at0 + row * step] = c[e];
-                }
+                write_result(a, t.z, c, rb, cb, t.lane, keep, rate);
             }
     }
 };
@@ -308,7 +187,7 @@ Space space_for(char *base, int count, int64_t rows, int64_t cols)
     Space s;
     const int64_t sums = (odl::ceil_div((int64_t)count * norm_blocks(rows * cols) * 8, 256)) * 256;
     const int64_t xb = panel_bytes(mp, np), ab = panel_bytes(mp, mp);
-    s.batch_bytes = 4 * xb + 2 * ab;
+    s.batch_bytes = slim_fits(rows, cols) ? (int64_t)slim_bytes(rows, cols) : 4 * xb + 2 * ab;
     char *at      = base + sums;
     s.sums        = reinterpret_cast<double *>(base);
     for (int i = 0; i < 2; ++i)
@@ -366,8 +245,13 @@ int run_group(const Matrices &mat, int count, int steps, float a, float b, float
     const bool tall  = mat.rows > mat.cols;
     const int64_t m = std::min(mat.rows, mat.cols), n = std::max(mat.rows, mat.cols), mp = padded(m), np = padded(n);
     const int parts = norm_blocks(mat.rows * mat.cols);
-    muon_norm_kernel<<<dim3((unsigned)parts, (unsigned)count), dim3(kBlock), 0, st>>>(mat, s.sums);
-    ODL_LAUNCH_CHECK();
+    if (!slim_whole(mat.rows, mat.cols))
+    {
+        muon_norm_kernel<<<dim3((unsigned)parts, (unsigned)count), dim3(kBlock), 0, st>>>(mat, s.sums);
+        ODL_LAUNCH_CHECK();
+    }
+    if (slim_fits(mat.rows, mat.cols))
+        return slim_run(mat, count, Settings{steps, a, b, c, eps, keep, rate}, s.sums, parts, s.xr[0].base, st);
     const int64_t rp = tall ? np : mp, cp = tall ? mp : np;
     muon_prepare_kernel<<<dim3((unsigned)(cp / 64), (unsigned)(rp / 64), (unsigned)count), dim3(kBlock), 0, st>>>(
         mat, s.sums, parts, (double)eps, tall ? s.xt[0] : s.xr[0], tall ? s.xr[0] : s.xt[0], s.batch_bytes);

@@ -64,10 +64,23 @@ inline int64_t padded(int64_t n)
     return ceil_div(n, t) * t;
 }
 
-__device__ inline void split_value(float y, _Float16 &hi, _Float16 &lo)
+// Two values into hi and lo, both rounded to nearest. The mixed-precision multiply-add takes a float16 as it lies in half a
+// register: x - hi is one instruction, where converting hi back first would take two.
+typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+__device__ inline void split_pair(float x, float y, unsigned &hi, unsigned &lo)
 {
-    hi = (_Float16)y;
-    lo = (_Float16)(y - (float)hi);
+    hi = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){x, y}, half2));
+    float rx, ry;
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel_hi:[1,0,0]" : "=v"(rx) : "v"(hi), "v"(x));
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(ry) : "v"(hi), "v"(y));
+    lo = __builtin_bit_cast(unsigned, __builtin_convertvector((f32x2){rx, ry}, half2));
+}
+// hi + lo
+__device__ inline void join_pair(unsigned hi, unsigned lo, float &x, float &y)
+{
+    asm("v_fma_mix_f32 %0, %1, 1.0, %2 op_sel_hi:[1,0,1]" : "=v"(x) : "v"(hi), "v"(lo));
+    asm("v_fma_mix_f32 %0, %1, 1.0, %2 op_sel:[1,0,1] op_sel_hi:[1,0,1]" : "=v"(y) : "v"(hi), "v"(lo));
 }
 
 // where lane `lane` keeps its 8 values (hi; lo follows 1024 bytes later) of block (row block rb, contraction block kb)
@@ -76,28 +89,29 @@ __device__ inline char *fragment(const Panel &p, int64_t rb, int64_t kb, int lan
     return p.base + (rb * p.kb + kb) * kBlockBytes + lane * 16;
 }
 
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 __device__ inline void store_fragment(const Panel &p, int64_t rb, int64_t kb, int lane, const float *v)
 {
-    half8 hi, lo;
+    u32x4 hi, lo;
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 4; ++i)
     {
-        _Float16 h, l;
-        split_value(v[i], h, l);
+        unsigned h, l;
+        split_pair(v[2 * i], v[2 * i + 1], h, l);
         hi[i] = h, lo[i] = l;
     }
     char *at = fragment(p, rb, kb, lane);
-    *reinterpret_cast<half8 *>(at)        = hi;
-    *reinterpret_cast<half8 *>(at + 1024) = lo;
+    *reinterpret_cast<u32x4 *>(at)        = hi;
+    *reinterpret_cast<u32x4 *>(at + 1024) = lo;
 }
 
 __device__ inline void load_fragment(const Panel &p, int64_t rb, int64_t kb, int lane, float *v)
 {
     const char *at = fragment(p, rb, kb, lane);
-    const half8 hi = *reinterpret_cast<const half8 *>(at), lo = *reinterpret_cast<const half8 *>(at + 1024);
+    const u32x4 hi = *reinterpret_cast<const u32x4 *>(at), lo = *reinterpret_cast<const u32x4 *>(at + 1024);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        v[i] = (float)hi[i] + (float)lo[i];
+    for (int i = 0; i < 4; ++i)
+        join_pair(hi[i], lo[i], v[2 * i], v[2 * i + 1]);
 }
 
 // 16 bytes a lane from a buffer into LDS: lane i's data lands at lds_byte_address + 16 * i. An instruction and not the

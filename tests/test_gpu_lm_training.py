@@ -317,7 +317,7 @@ def schulz_bar(steps, coef=COEF):
 
 
 MATRICES = [(1, 1), (1, 7), (7, 1), (2, 3), (31, 33), (64, 64), (65, 100), (100, 65), (97, 97), (128, 300), (300, 128), (257, 769), (769, 257),
-            (770, 800), (1030, 1030), (33, 4099), (2100, 2100)]
+            (770, 800), (1030, 1030), (33, 4099), (2100, 2100), (64, 4096), (4096, 128), (128, 513), (513, 60), (120, 1000), (129, 4000)]
 
 
 @pytest.mark.parametrize("shape", MATRICES)
@@ -341,7 +341,7 @@ def test_newton_schulz_brings_singular_values_near_one(capi):
     assert float((core - torch.diag(core.diagonal())).norm()) < 1e-2 and float((o - u @ core @ v.t()).norm()) < 1e-2
 
 
-@pytest.mark.parametrize("batch,rows,cols", [(2, 40, 50), (3, 130, 70), (33, 65, 64), (5, 1, 9)])
+@pytest.mark.parametrize("batch,rows,cols", [(2, 40, 50), (3, 130, 70), (33, 65, 64), (5, 1, 9), (3, 140, 600), (34, 150, 131)])
 def test_a_batch_gives_what_its_matrices_give(capi, batch, rows, cols):
     g = torch.randn(batch, rows, cols, device="cuda", generator=gen(batch))
     got = capi.newton_schulz(g)
