@@ -173,6 +173,8 @@ struct Space
     double *sums;
     Panel xr[2], xt[2], a, b;
     int64_t batch_bytes;
+    Cut gram, poly, step;
+    void *parts;  // of a product whose contraction is cut
     size_t bytes;
 };
 
@@ -195,6 +197,18 @@ Space space_for(char *base, int count, int64_t rows, int64_t cols)
     s.a     = Panel{at + 4 * xb, mp / 16};
     s.b     = Panel{at + 4 * xb + ab, mp / 16};
     s.bytes = (size_t)(sums + count * s.batch_bytes);
+    s.parts = base + s.bytes;
+    if (!slim_fits(rows, cols))
+    {
+        const int kb_m = contraction_blocks(std::min(rows, cols)), kb_n = contraction_blocks(std::max(rows, cols));
+        const double square = 2.0 * (double)count * mp * (mp + 64), whole = 4.0 * (double)count * mp * np;
+        // a step passes on what its sums round, up to 3.4 times: long ones are kept apart (4096 x 4096, against 64 bits: 6.5e-6
+        // with one set of accumulators, 3.0e-6 for float32 products in quarters)
+        const bool exact = kb_m > 64;
+        s.gram = pick_cut(mp, mp, true, count, kb_n, true, square, exact), s.poly = pick_cut(mp, mp, true, count, kb_m, true, square, exact);
+        s.step = pick_cut(mp, np, false, count, kb_m, true, whole, exact);
+        s.bytes += std::max({part_bytes(s.gram, mp, mp, count), part_bytes(s.poly, mp, mp, count), part_bytes(s.step, mp, np, count)});
+    }
     return s;
 }
 
@@ -257,7 +271,6 @@ int run_group(const Matrices &mat, int count, int steps, float a, float b, float
         mat, s.sums, parts, (double)eps, tall ? s.xt[0] : s.xr[0], tall ? s.xr[0] : s.xt[0], s.batch_bytes);
     ODL_LAUNCH_CHECK();
     const int kb_m = contraction_blocks(m), kb_n = contraction_blocks(n);
-    const Cut gram = pick_cut(mp, mp, true, count, kb_n), poly = pick_cut(mp, mp, true, count, kb_m), step = pick_cut(mp, np, false, count, kb_m);
     for (int k = 0; k < steps; ++k)
     {
         const Panel xr = s.xr[k & 1], xt = s.xt[k & 1];
@@ -265,18 +278,18 @@ int run_group(const Matrices &mat, int count, int steps, float a, float b, float
         g.batch = count, g.a_batch = g.b_batch = s.batch_bytes;
         g.symmetric = 1;
         g.a = xr, g.b = xr, g.nkb = kb_n;
-        if (int rc = launch_gemm(g, mp, mp, gram, SymmetricEpilogue{s.a, Panel{nullptr, 0}, s.batch_bytes, 1.f / kScale, 0.f}, st))
+        if (int rc = launch_whole_gemm(g, mp, mp, s.gram, s.parts, SymmetricEpilogue{s.a, Panel{nullptr, 0}, s.batch_bytes, 1.f / kScale, 0.f}, st))
             return rc;
         g.a = s.a, g.b = s.a, g.nkb = kb_m;
-        if (int rc = launch_gemm(g, mp, mp, poly, SymmetricEpilogue{s.b, s.a, s.batch_bytes, c / kScale, b}, st))
+        if (int rc = launch_whole_gemm(g, mp, mp, s.poly, s.parts, SymmetricEpilogue{s.b, s.a, s.batch_bytes, c / kScale, b}, st))
             return rc;
         g.symmetric = 0;
         g.a = s.b, g.b = xt;
         int rc;
         if (k + 1 < steps)
-            rc = launch_gemm(g, mp, np, step, StepEpilogue{xt, s.xt[(k + 1) & 1], s.xr[(k + 1) & 1], s.batch_bytes, 1.f / kScale, a}, st);
+            rc = launch_whole_gemm(g, mp, np, s.step, s.parts, StepEpilogue{xt, s.xt[(k + 1) & 1], s.xr[(k + 1) & 1], s.batch_bytes, 1.f / kScale, a}, st);
         else
-            rc = launch_gemm(g, mp, np, step, LastEpilogue{xt, s.batch_bytes, 1.f / kScale / kScale, a / kScale, mat, keep, rate}, st);
+            rc = launch_whole_gemm(g, mp, np, s.step, s.parts, LastEpilogue{xt, s.batch_bytes, 1.f / kScale / kScale, a / kScale, mat, keep, rate}, st);
         if (rc)
             return rc;
     }

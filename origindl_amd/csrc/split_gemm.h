@@ -15,6 +15,9 @@
 // of 16 bytes a lane, a fragment is one ds_read_b128 without bank conflicts, and rows, columns and contraction values past
 // the matrix are zeros in memory, so the product's loop has no edges.
 //
+// Sums. Every product added to an accumulator rounds it once more, the small cross terms too. Where registers allow (all tiles
+// but 256 x 256) the cross terms have accumulators of their own, which join the others at the end: a third of the roundings.
+//
 // The product. A workgroup holds a BM x BN tile; four stages of one contraction block each travel into LDS by direct loads
 // (no registers), queued four stages ahead; fragments of the next block are read while the present block multiplies. A
 // stage's three products use 4 fragments a pair of blocks where a plain float16 product reads 2 for one, so LDS needs only
@@ -302,6 +305,18 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void split_gemm_kernel(const GemmAr
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 acc[i][j][e] = 0.f;
+    constexpr bool kApart = BM * BN < 256 * 256;
+    f32x16 cross[kApart ? MI : 1][kApart ? NI : 1];
+    if constexpr (kApart)
+    {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    cross[i][j][e] = 0.f;
+    }
     // One stage. A's next fragment is read under the products of the present one; before the last block's products comes the
     // round's only barrier: every wave has read all of stage kb, whose slot takes stage kb + kStages, and stage kb + 1 has
     // landed, whose first fragments are read under those products. P: which of the two A fragments the stage begins with.
@@ -326,10 +341,16 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void split_gemm_kernel(const GemmAr
             const FragA &a = fa[(A0 + i) & 1];
 #pragma unroll
             for (int j = 0; j < NI; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, fb[P].l[j], acc[i][j], 0, 0, 0);
+            {
+                f32x16 &c = kApart ? cross[kApart ? i : 0][kApart ? j : 0] : acc[i][j];
+                c         = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, fb[P].l[j], c, 0, 0, 0);
+            }
 #pragma unroll
             for (int j = 0; j < NI; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.l, fb[P].h[j], acc[i][j], 0, 0, 0);
+            {
+                f32x16 &c = kApart ? cross[kApart ? i : 0][kApart ? j : 0] : acc[i][j];
+                c         = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.l, fb[P].h[j], c, 0, 0, 0);
+            }
 #pragma unroll
             for (int j = 0; j < NI; ++j)
                 acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a.h, fb[P].h[j], acc[i][j], 0, 0, 0);
@@ -350,6 +371,16 @@ __global__ __launch_bounds__(64 * WM *WN, 2) void split_gemm_kernel(const GemmAr
     }
     wait_loads_and_lds<0>();  // no load is under way into LDS that the epilogue writes
     barrier();
+    if constexpr (kApart)
+    {
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    acc[i][j][e] += cross[i][j][e];
+    }
     epilogue(t, acc);
 }
 
@@ -386,21 +417,23 @@ __global__ __launch_bounds__(64 * kDirectWaves, 2) void split_gemm_direct_kernel
             f.bl[i] = __builtin_bit_cast(half8, __builtin_amdgcn_raw_buffer_load_b128(rb, off, (int)(i * b_rb) + 1024, 0));
         }
     };
-    f32x16 acc[2][2];
+    f32x16 acc[2][2], cross[2][2];
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
-        acc[0][0][e] = acc[0][1][e] = acc[1][0][e] = acc[1][1][e] = 0.f;
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+            acc[i >> 1][i & 1][e] = cross[i >> 1][i & 1][e] = 0.f;
     const auto multiply = [&](const Frags &f) {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bl[j], acc[i][j], 0, 0, 0);
+                cross[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.ah[i], f.bl[j], cross[i][j], 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
             for (int j = 0; j < 2; ++j)
-                acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.al[i], f.bh[j], acc[i][j], 0, 0, 0);
+                cross[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f.al[i], f.bh[j], cross[i][j], 0, 0, 0);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -423,7 +456,7 @@ __global__ __launch_bounds__(64 * kDirectWaves, 2) void split_gemm_direct_kernel
 #pragma unroll
         for (int q = 0; q < 4; ++q)
         {
-            const f32x16 &c = acc[b >> 1][b & 1];
+            const f32x16 c = acc[b >> 1][b & 1] + cross[b >> 1][b & 1];
             mine[b * 256 + q * 64] = f32x4{c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]};
         }
     __syncthreads();
@@ -458,9 +491,10 @@ struct Cut
 // TFLOP/s at which many of them run into the chip's power limit (long symmetric products lower: their tiles share less),
 // and microseconds a round of tiles spends outside its loop. Large tiles read their operands less often and leave compute
 // units idle in a short last round. Runs of the contraction (may_split) cost a pass over the partial results: out_bytes
-// written per run, read once. For example 4096 x 4096 x 4096: 323 us with 256 x 256, 325 with 256 x 128, 333 with 128 x 128, 404
+// written per run, read once. exact: only tiles with accumulators apart for the cross terms. For example 4096 x 4096 x 4096: 323 us with 256 x 256, 325 with 256 x 128, 333 with 128 x 128, 404
 // with 64 x 64; 1024 x 1024 x 1024: 52, 29, 19 and 8.6 us.
-inline Cut pick_cut(int64_t rows_pad, int64_t cols_pad, bool symmetric, int64_t batch, int nkb, bool may_split = false, double out_bytes = 0)
+inline Cut pick_cut(int64_t rows_pad, int64_t cols_pad, bool symmetric, int64_t batch, int nkb, bool may_split = false, double out_bytes = 0,
+                    bool exact = false)
 {
     struct Option
     {
@@ -475,10 +509,10 @@ inline Cut pick_cut(int64_t rows_pad, int64_t cols_pad, bool symmetric, int64_t 
     double best_cost = 0;
     for (const Option &o : options)
     {
-        if (rows_pad % o.bm || cols_pad % o.bn || (symmetric && o.bm != o.bn))
+        if (rows_pad % o.bm || cols_pad % o.bn || (symmetric && o.bm != o.bn) || (exact && o.bm * o.bn == 256 * 256))
             continue;
         const int64_t tm = rows_pad / o.bm, tn = cols_pad / o.bn, tiles = batch * (symmetric ? tm * (tm + 1) / 2 : tm * tn);
-        for (int s = 1; s <= (may_split ? 32 : 1) && (s == 1 || nkb / s >= 16); ++s)
+        for (int s = 1; s <= (may_split ? 32 : 1) && (s == 1 || nkb / s >= 8); ++s)
         {
             const int kb = s == 1 ? nkb : (int)ceil_div(nkb, 2 * s) * 2;
             if (s > 1 && (int64_t)(s - 1) * kb >= nkb)
@@ -488,7 +522,7 @@ inline Cut pick_cut(int64_t rows_pad, int64_t cols_pad, bool symmetric, int64_t 
             double cost = kb * ((double)full * o.resident * o.full + last);
             cost = std::max(cost, (double)work * kb * o.bm * o.bn * 32.0 / (symmetric ? o.symmetric_rate : o.rate) / 1e6) + o.fixed * (double)(full + (rest != 0));
             if (s > 1)
-                cost += 3.0 + out_bytes * (s + 1) / 4e6;
+                cost += 5.0 + out_bytes * (s + 1) / 4e6;
             if (best_cost == 0 || cost < best_cost)
                 best = Cut{o.bm, o.bn, s, kb}, best_cost = cost;
         }
@@ -496,11 +530,68 @@ inline Cut pick_cut(int64_t rows_pad, int64_t cols_pad, bool symmetric, int64_t 
     return best;
 }
 
-template <class Epilogue>
-inline int launch_gemm(GemmArgs g, int64_t rows_pad, int64_t cols_pad, const Cut &cut, const Epilogue &e, hipStream_t st)
+// Where a run of the contraction leaves its accumulators: [product][row block][column block][run], 32 x 32 each as a wave
+// holds them.
+struct PartEpilogue
 {
-    g.tiles_m = (int)(rows_pad / cut.bm), g.tiles_n = (int)(cols_pad / cut.bn), g.xcds = chip().xcds;
-    g.splits = cut.splits, g.split_kb = cut.split_kb;
+    f32x4 *parts;
+    int64_t row_blocks, col_blocks;
+    int splits;
+    __device__ f32x4 *at(int z, int64_t rb, int64_t cb) const { return parts + ((z * row_blocks + rb) * col_blocks + cb) * splits * 256; }
+    template <class T, class Acc>
+    __device__ void operator()(const T &t, Acc &acc) const
+    {
+#pragma unroll
+        for (int mi = 0; mi < T::MI; ++mi)
+#pragma unroll
+            for (int ni = 0; ni < T::NI; ++ni)
+            {
+                const f32x16 &c = acc[mi][ni];
+                f32x4 *out      = at(t.z, t.row_block(mi), t.col_block(ni)) + t.split * 256 + t.lane;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    out[q * 64] = f32x4{c[4 * q], c[4 * q + 1], c[4 * q + 2], c[4 * q + 3]};
+            }
+    }
+};
+
+// The runs' accumulators added up in order, then the epilogue: the second launch of a product whose contraction is cut, on
+// 64 x 64 tiles whatever the first one's were (many workgroups, each a short chain of loads).
+template <class Epilogue>
+__global__ __launch_bounds__(256) void split_gemm_finish_kernel(const GemmArgs g, const PartEpilogue parts, const Epilogue epilogue)
+{
+    __shared__ __attribute__((aligned(16))) char lds[4 * 32 * 33 * 4];
+    Tile<64, 64, 2, 2> t;
+    tile_of(g, t.z, t.split, t.tm, t.tn);
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    t.lane = threadIdx.x & 63, t.wm = wave >> 1, t.wn = wave & 1, t.lds = lds;
+    const f32x4 *in = parts.at(t.z, t.row_block(0), t.col_block(0)) + t.lane;
+    f32x16 acc[1][1];
+#pragma unroll
+    for (int e = 0; e < 16; ++e)
+        acc[0][0][e] = 0.f;
+#pragma unroll 8
+    for (int s = 0; s < parts.splits; ++s)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+        {
+            const f32x4 v = in[s * 256 + q * 64];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                acc[0][0][4 * q + e] += v[e];
+        }
+    epilogue(t, acc);
+}
+
+// bytes of the runs' accumulators
+inline size_t part_bytes(const Cut &cut, int64_t rows_pad, int64_t cols_pad, int64_t batch)
+{
+    return cut.splits > 1 ? (size_t)cut.splits * (size_t)(batch * rows_pad * cols_pad) * 4 : 0;
+}
+
+template <class Epilogue>
+inline int launch_tiles(const GemmArgs &g, const Cut &cut, const Epilogue &e, hipStream_t st)
+{
     const int64_t blocks = g.blocks();
     ODL_REQUIRE(blocks < ((int64_t)1 << 31), "product of too many tiles");
     if (blocks == 0 || g.nkb == 0)
@@ -516,6 +607,38 @@ inline int launch_gemm(GemmArgs g, int64_t rows_pad, int64_t cols_pad, const Cut
         split_gemm_kernel<128, 128, 2, 2, Epilogue><<<grid, dim3(256), 0, st>>>(g, e);
     else
         split_gemm_direct_kernel<Epilogue><<<grid, dim3(64 * kDirectWaves), 0, st>>>(g, e);
+    ODL_LAUNCH_CHECK();
+    return ODL_OK;
+}
+
+inline GemmArgs cut_args(GemmArgs g, int64_t rows_pad, int64_t cols_pad, const Cut &cut)
+{
+    g.tiles_m = (int)(rows_pad / cut.bm), g.tiles_n = (int)(cols_pad / cut.bn), g.xcds = chip().xcds;
+    g.splits = cut.splits, g.split_kb = cut.split_kb;
+    return g;
+}
+
+// the epilogue sees t.split, the run of the contraction its accumulators cover
+template <class Epilogue>
+inline int launch_gemm(const GemmArgs &g, int64_t rows_pad, int64_t cols_pad, const Cut &cut, const Epilogue &e, hipStream_t st)
+{
+    return launch_tiles(cut_args(g, rows_pad, cols_pad, cut), cut, e, st);
+}
+
+// the epilogue sees the whole sums: with runs of the contraction (parts: part_bytes) in a second launch
+template <class Epilogue>
+inline int launch_whole_gemm(const GemmArgs &args, int64_t rows_pad, int64_t cols_pad, const Cut &cut, void *parts, const Epilogue &e, hipStream_t st)
+{
+    GemmArgs g = cut_args(args, rows_pad, cols_pad, cut);
+    if (cut.splits == 1)
+        return launch_tiles(g, cut, e, st);
+    const PartEpilogue p{static_cast<f32x4 *>(parts), rows_pad / 32, cols_pad / 32, cut.splits};
+    if (int rc = launch_tiles(g, cut, p, st))
+        return rc;
+    g = cut_args(args, rows_pad, cols_pad, Cut{64, 64, 1, args.nkb});
+    const int64_t blocks = g.blocks();
+    ODL_REQUIRE(blocks < ((int64_t)1 << 31), "product of too many tiles");
+    split_gemm_finish_kernel<Epilogue><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(g, p, e);
     ODL_LAUNCH_CHECK();
     return ODL_OK;
 }
