@@ -502,7 +502,7 @@ inline Cut pick_cut(int64_t rows_pad, int64_t cols_pad, bool symmetric, int64_t 
         double alone, full, rate, symmetric_rate, fixed;
     };
     static const Option options[] = {{256, 256, 1, 0.80, 0.80, 425, 425, 12.0}, {256, 128, 1, 0.46, 0.46, 405, 405, 7.0},
-                                     {128, 256, 1, 0.46, 0.46, 405, 405, 7.0}, {128, 128, 2, 0.30, 0.26, 400, 400, 4.0},
+                                     {128, 256, 1, 0.46, 0.46, 405, 405, 7.0}, {128, 128, 2, 0.37, 0.26, 400, 400, 4.0},
                                      {64, 64, 2, 0.107, 0.085, 330, 230, 2.0}};
     const int cus = device_cus();
     Cut best{64, 64, 1, nkb};
