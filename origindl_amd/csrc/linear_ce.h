@@ -99,7 +99,7 @@ struct Problem
 // estimates of both cross at about 6 million weights.
 inline bool few_rows(int64_t N, int64_t K, int64_t V)
 {
-    return N <= 64 && K * V >= 6000000;
+    return N <= 256 && K * V >= 6000000;
 }
 size_t few_forward_bytes(int64_t N, int64_t K, int64_t V);
 size_t few_backward_bytes(int64_t N, int64_t K, int64_t V);

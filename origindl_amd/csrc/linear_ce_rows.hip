@@ -1,17 +1,21 @@
-// The output layer with its loss for up to 64 rows: scoring a few positions, small batches.
+// The output layer with its loss for up to 256 rows over large weights: scoring a few positions, small batches.
 //
-// What bounds it: the bytes of w. A pass over w [V, K] multiplies 2N operations per element of 4 bytes, which the float32 matrix
-// instructions do in less time than memory delivers w (N = 64: as fast). So nothing is laid out first: w streams once from
-// where it lies into float32 matrix instructions (v_mfma_f32_32x32x2), per pass:
-//   forward    one pass: logits of 128 entries a workgroup, their maximum and sum of powers in its epilogue
-//   backward   one pass for the logits again, whose epilogue writes d = softmax - one-hot ([V][N] floats: the weights' size
-//              times N / K) and gb; one pass for gx = d.w, in runs of the vocabulary; gw = d^T.x writes its size once.
+// What bounds it: the bytes of w. So nothing is laid out first: w streams once from where it lies through the registers into
+// the matrix instructions, per pass:
+//   forward    one pass: logits of 128 (64) entries a workgroup, their maximum and sum of powers in its epilogue
+//   backward   one pass for the logits again, whose epilogue writes d = softmax - one-hot (the weights' size times 3N / K) and
+//              gb; one pass for gx = d.w, in runs of the vocabulary; gw = d^T.x writes its size once.
+//
+// Mathematics. A float32 number is the sum of three bfloat16 numbers, its first, second and third eight bits, cut off without
+// rounding: exact. Of the nine products of two such sums the six of at least 2^-16 of the whole are formed by bfloat16 matrix
+// instructions (v_mfma_f32_32x32x16_bf16), exact in float32, and summed there: what is left out is under 2^-23 of |a||b|. No
+// scale is needed, as bfloat16 has float32's exponents, and so no pass over w to find one. Six products take 0.38 of the float32
+// matrix instruction's time: memory stays what bounds a pass up to about 160 rows.
 //
 // Both products with w are one kernel: w is [out][contraction] for the logits of a [V, K] weight and [contraction][out] for its
-// gx, and the other way round for a [K, V] weight. Eight waves share a tile of 128 outputs, each takes an eighth of the
-// contraction, 8 values a step: lanes of the lower half-wave the first four, of the upper half the others, so that w and the
-// small operand both arrive as 16 bytes a lane. The small operand lies as q[contraction / 4][rows][4], zeros past the ends and
-// in rows that do not count.
+// gx, and the other way round for a [K, V] weight. Eight waves share a tile of outputs, each takes an eighth of the contraction,
+// 16 values a step, splits what it read and multiplies it with the small operand (x or d), which lies split, in the order of
+// the instructions' lanes.
 #include <algorithm>
 
 #include "linear_ce.h"
@@ -21,139 +25,226 @@ namespace
 using namespace odl::linear_ce;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));  // rows of w need not start on 16 bytes
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kWaves = 8, kTile = 128;
+constexpr int kWaves = 8;
+constexpr int kFragment = 3 * 64;  // u32x4 of a block of 32 rows x 16 contraction values: three parts, 16 bytes a lane
 
-// x as q[k / 4][rows][4]; rows = 32 or 64. Also clears the ticket of the joining launch.
-__global__ __launch_bounds__(kBlock) void ce_rows_prepare_kernel(const float *__restrict__ x, int64_t K, const Labels labels, int rows, int64_t quads,
-                                                                 f32x4 *__restrict__ q, float *saved)
+// eight float32 into their first, second and third eight bits
+__device__ inline void split3(const float *v, u32x4 *part)
+{
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+    {
+        const float a0 = v[2 * i], b0 = v[2 * i + 1];
+        const unsigned a = __float_as_uint(a0), b = __float_as_uint(b0);
+        const float a1 = a0 - __uint_as_float(a & 0xffff0000u), b1 = b0 - __uint_as_float(b & 0xffff0000u);
+        const unsigned am = __float_as_uint(a1), bm = __float_as_uint(b1);
+        const float a2 = a1 - __uint_as_float(am & 0xffff0000u), b2 = b1 - __uint_as_float(bm & 0xffff0000u);
+        // the upper halves of both, the first value in the lower half
+        part[0][i] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+        part[1][i] = __builtin_amdgcn_perm(bm, am, 0x07060302u);
+        part[2][i] = __builtin_amdgcn_perm(__float_as_uint(b2), __float_as_uint(a2), 0x07060302u);
+    }
+}
+
+__device__ inline f32x16 mfma(const u32x4 &a, const u32x4 &b, const f32x16 &c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// c += a . b: the small products first
+__device__ inline void multiply(f32x16 &c, const u32x4 *a, const u32x4 *b)
+{
+    c = mfma(a[0], b[2], c);
+    c = mfma(a[2], b[0], c);
+    c = mfma(a[1], b[1], c);
+    c = mfma(a[0], b[1], c);
+    c = mfma(a[1], b[0], c);
+    c = mfma(a[0], b[0], c);
+}
+
+__device__ inline void store3(u32x4 *at, const float *v, int lane)
+{
+    u32x4 part[3];
+    split3(v, part);
+#pragma unroll
+    for (int p = 0; p < 3; ++p)
+        at[p * 64 + lane] = part[p];
+}
+
+// x split: by_n as the small operand of the logits, [K / 16][blocks of 32 rows]; by_k as an operand of gw, rows of K, [K / 32][rows
+// / 16] (null: not wanted). A wave makes one fragment of each. Also clears the ticket of the joining launch.
+__global__ __launch_bounds__(kBlock) void ce_rows_prepare_kernel(const float *__restrict__ x, int64_t K, const Labels labels, int blocks_n, int64_t groups,
+                                                                 int64_t blocks_k, u32x4 *__restrict__ by_n, u32x4 *__restrict__ by_k, float *saved)
 {
     if (saved && blockIdx.x == 0 && threadIdx.x == 0)
         reinterpret_cast<int *>(saved)[kTicket] = 0;
-    const int64_t at = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-    if (at >= quads * rows)
-        return;
-    // consecutive threads take consecutive quads of one row: x is read in whole lines
-    const int64_t n = at / quads, kq = at - n * quads;
-    f32x4 v = {0.f, 0.f, 0.f, 0.f};
-    if (labels(n) >= 0)
+    const int lane = threadIdx.x & 63;
+    const int64_t unit = (int64_t)blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6);
+    float v[8];
+    if (unit < groups * blocks_n)
     {
+        const int64_t g = unit / blocks_n, n = (unit - g * blocks_n) * 32 + (lane & 31), k = g * 16 + (lane >> 5) * 8;
+        const bool counts = labels(n) >= 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (kq * 4 + e < K)
-                v[e] = x[n * K + kq * 4 + e];
+        for (int e = 0; e < 8; ++e)
+            v[e] = counts && k + e < K ? x[n * K + k + e] : 0.f;
+        store3(by_n + unit * kFragment, v, lane);
     }
-    q[kq * rows + n] = v;
+    if (by_k && unit < blocks_k * blocks_n * 2)
+    {
+        const int64_t kb = unit / (blocks_n * 2), k = kb * 32 + (lane & 31), n0 = (unit - kb * blocks_n * 2) * 16 + (lane >> 5) * 8;
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            v[e] = k < K && labels(n0 + e) >= 0 ? x[(n0 + e) * K + k] : 0.f;
+        store3(by_k + unit * kFragment, v, lane);
+    }
 }
 
 struct Stream
 {
     const float *w;
     int64_t ld, outs, contraction;
-    const f32x4 *q;      // [groups * 2][NB * 32]
-    int64_t groups;      // steps of 8 contraction values
-    int64_t wave_groups; // steps of one wave
+    const u32x4 *q;       // the small operand, [groups][blocks_n]
+    int blocks_n;         // its blocks of 32 rows; a workgroup takes NB of them
+    int64_t groups;       // steps of 16 contraction values
+    int64_t wave_groups;  // steps of one wave
 };
 
-// OUT_ROWS: w is [out][contraction], else [contraction][out]. The epilogue is called by the first four waves with block m of
-// the tile: element 4q + e of s[nb] is row 8q + 4 * (lane / 32) + e of the block, column nb * 32 + lane % 32; a block's row r
-// is output 32m + r of the tile (OUT_ROWS) or 4r + m.
-template <int NB, bool OUT_ROWS, class Epilogue>
+// OUT_ROWS: w is [out][contraction], else [contraction][out]. A workgroup has 32 * VB outputs and 32 * NB rows; output of row r of
+// block m: 32m + r (OUT_ROWS) or VB * r + m. The epilogue is called by all waves; waves m < VB hold block m, element 4q + e of
+// s[nb] being row 8q + 4 * (lane / 32) + e, column nb * 32 + lane % 32.
+template <int VB, int NB, bool OUT_ROWS, class Epilogue>
 __global__ __launch_bounds__(64 * kWaves, 2) void ce_stream_kernel(const Stream a, const Epilogue epilogue)
 {
-    __shared__ f32x4 lds[kWaves * 4 * 256];
+    typedef float wide __attribute__((ext_vector_type(VB), aligned(4)));   // rows of w need not start on 16 bytes
+    typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+    constexpr int kTile = 32 * VB, kReduce = kWaves * VB * 4096, kRows = kTile * (32 * NB + 1) * 4;
+    __shared__ __attribute__((aligned(16))) char lds[kReduce > kRows ? kReduce : kRows];
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63, half = lane >> 5, col = lane & 31;
-    const int64_t o0 = (int64_t)blockIdx.x * kTile;
-    f32x16 acc[4][NB];
+    // workgroups with the same part of w are neighbours
+    const unsigned per_tile = (unsigned)(a.blocks_n / NB);
+    const unsigned tile     = blockIdx.x / per_tile;
+    const int nb0           = (int)(blockIdx.x - tile * per_tile) * NB;
+    const int64_t o0        = (int64_t)tile * kTile;
+    f32x16 acc[VB][NB];
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+    for (int m = 0; m < VB; ++m)
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 acc[m][nb][e] = 0.f;
+    const int64_t first = ((int64_t)blockIdx.y * kWaves + wave) * a.wave_groups, last = min(first + a.wave_groups, a.groups);
+    const int64_t whole = a.outs >= VB || OUT_ROWS ? min(last, a.contraction / 16) : first;
+    // In the last tile a lane past the outputs reads what lies in reach instead (its outputs are nobody's); of outputs that
+    // straddle the end it reads the last VB and moves them to their places.
+    const int64_t o_lane = o0 + col * VB, shift = OUT_ROWS ? 0 : o_lane + VB - a.outs;
+    const bool straddles = !OUT_ROWS && o0 + kTile > a.outs;
+    const float *w[VB];
+#pragma unroll
+    for (int m = 0; m < VB; ++m)
+        w[m] = OUT_ROWS ? a.w + min(o0 + 32 * m + col, a.outs - 1) * a.ld + half * 8 : a.w + (int64_t)(half * 8) * a.ld + (shift > 0 ? a.outs - VB : o_lane);
+    const u32x4 *q = a.q + (int64_t)nb0 * kFragment + lane;
     struct Step
     {
-        f32x4 w[4], q[NB];
+        float v[VB][8];  // block m's eight contraction values
     };
-    const f32x4 *q = a.q + (int64_t)half * NB * 32 + col;
-    const int64_t first = ((int64_t)blockIdx.y * kWaves + wave) * a.wave_groups, last = min(first + a.wave_groups, a.groups);
-    const int64_t whole = a.outs >= 4 || OUT_ROWS ? min(last, a.contraction / 8) : first;
-    // In the last tile a lane past the outputs reads what lies in reach instead (its outputs are nobody's); of four outputs that
-    // straddle the end it reads the last four and moves them to their places.
-    const int64_t o_lane = o0 + col * 4, shift = OUT_ROWS ? 0 : o_lane + 4 - a.outs;
-    const float *w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        w[i] = OUT_ROWS ? a.w + min(o0 + 32 * i + col, a.outs - 1) * a.ld + half * 4 : a.w + (int64_t)(half * 4 + i) * a.ld + (shift > 0 ? a.outs - 4 : o_lane);
-    const int64_t w_step = OUT_ROWS ? 8 : 8 * a.ld;
     const auto load = [&](int64_t g, Step &s) {
         const int64_t at = min(g, whole - 1);  // past the wave's last whole step: that one again, multiplied by nobody
+        if constexpr (OUT_ROWS)
+        {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            s.w[i] = *reinterpret_cast<const f32x4u *>(w[i] + at * w_step);
+            for (int m = 0; m < VB; ++m)
+            {
+                const f32x4 lo = *reinterpret_cast<const f32x4u *>(w[m] + at * 16), hi = *reinterpret_cast<const f32x4u *>(w[m] + at * 16 + 4);
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-            s.q[nb] = q[at * 2 * NB * 32 + nb * 32];
+                for (int e = 0; e < 4; ++e)
+                    s.v[m][e] = lo[e], s.v[m][4 + e] = hi[e];
+            }
+        }
+        else
+        {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+            {
+                const wide r = *reinterpret_cast<const wide *>(w[0] + (at * 16 + e) * a.ld);
+#pragma unroll
+                for (int m = 0; m < VB; ++m)
+                    s.v[m][e] = r[m];
+            }
+        }
     };
-    // the contraction's last values, single loads with zeros past its end (and outputs fewer than four)
+    // the contraction's last values, single loads with zeros past its end (and outputs fewer than VB)
     const auto load_guarded = [&](int64_t g, Step &s) {
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-            s.q[nb] = q[g * 2 * NB * 32 + nb * 32];
+        for (int m = 0; m < VB; ++m)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < 8; ++e)
             {
-                const int64_t o = OUT_ROWS ? o0 + 32 * i + col : o0 + col * 4 + e, c = g * 8 + half * 4 + (OUT_ROWS ? e : i);
-                s.w[i][e] = o < a.outs && c < a.contraction ? a.w[OUT_ROWS ? o * a.ld + c : c * a.ld + o] : 0.f;
+                const int64_t o = OUT_ROWS ? o0 + 32 * m + col : o0 + col * VB + m, c = g * 16 + half * 8 + e;
+                s.v[m][e] = o < a.outs && c < a.contraction ? a.w[OUT_ROWS ? o * a.ld + c : c * a.ld + o] : 0.f;
             }
     };
-    const bool straddles = !OUT_ROWS && o0 + kTile > a.outs;
-    const auto multiply = [&](const Step &s, bool move) {
+    const auto load_q = [&](int64_t g, u32x4 (*b)[3]) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int p = 0; p < 3; ++p)
+                b[nb][p] = q[(g * a.blocks_n + nb) * kFragment + p * 64];
+    };
+    const auto step = [&](Step &s, const u32x4 (*b)[3], bool move) {
+        if (move)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+                for (int i = 1; i < VB; ++i)
+                    if (shift == i)
+                    {
+#pragma unroll
+                        for (int m = 0; m < VB; ++m)
+                            s.v[m][e] = m + i < VB ? s.v[m + i < VB ? m + i : m][e] : 0.f;
+                    }
+#pragma unroll
+        for (int m = 0; m < VB; ++m)
         {
-            f32x4 v = s.w[j];
-            if (move)
-            {
-                v = shift == 1 ? f32x4{v[1], v[2], v[3], 0.f} : v;
-                v = shift == 2 ? f32x4{v[2], v[3], 0.f, 0.f} : v;
-                v = shift == 3 ? f32x4{v[3], 0.f, 0.f, 0.f} : v;
-            }
+            u32x4 part[3];
+            split3(s.v[m], part);
 #pragma unroll
-            for (int m = 0; m < 4; ++m)
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb)
-                    acc[m][nb] = __builtin_amdgcn_mfma_f32_32x32x2f32(OUT_ROWS ? s.w[m][j] : v[m], s.q[nb][j], acc[m][nb], 0, 0, 0);
+            for (int nb = 0; nb < NB; ++nb)
+                multiply(acc[m][nb], part, b[nb]);
         }
     };
     if (first < whole)
     {
-        Step s0, s1, t0, t1;
-        load(first, s0), load(first + 1, s1);
-        for (int64_t g = first; g < whole; g += 4)
+        Step s0, s1;
+        u32x4 b[NB][3];
+        load(first, s0);
+        for (int64_t g = first; g < whole; g += 2)
         {
-            load(g + 2, t0), load(g + 3, t1);
-            multiply(s0, straddles);
+            load_q(g, b);
+            load(g + 1, s1);
+            step(s0, b, straddles);
             if (g + 1 < whole)
-                multiply(s1, straddles);
-            load(g + 4, s0), load(g + 5, s1);
-            if (g + 2 < whole)
-                multiply(t0, straddles);
-            if (g + 3 < whole)
-                multiply(t1, straddles);
+            {
+                load_q(g + 1, b);
+                load(g + 2, s0);
+                step(s1, b, straddles);
+            }
         }
     }
     for (int64_t g = max(first, whole); g < last; ++g)
     {
         Step s;
+        u32x4 b[NB][3];
+        load_q(g, b);
         load_guarded(g, s);
-        multiply(s, false);
+        step(s, b, false);
     }
-    // the waves' sums, one block of columns at a time; wave m < 4 adds up block m in the waves' order
+    // the waves' sums, one block of columns at a time; wave m < VB adds up block m in the waves' order
+    f32x4 *sums = reinterpret_cast<f32x4 *>(lds);
     f32x16 sum[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
@@ -161,59 +252,66 @@ __global__ __launch_bounds__(64 * kWaves, 2) void ce_stream_kernel(const Stream 
         if (nb)
             __syncthreads();
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
+        for (int m = 0; m < VB; ++m)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                lds[(wave * 4 + m) * 256 + i * 64 + lane] = f32x4{acc[m][nb][4 * i], acc[m][nb][4 * i + 1], acc[m][nb][4 * i + 2], acc[m][nb][4 * i + 3]};
+                sums[(wave * VB + m) * 256 + i * 64 + lane] = f32x4{acc[m][nb][4 * i], acc[m][nb][4 * i + 1], acc[m][nb][4 * i + 2], acc[m][nb][4 * i + 3]};
         __syncthreads();
-        if (wave < 4)
+        if (wave < VB)
         {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
             {
-                f32x4 v = lds[wave * 256 + i * 64 + lane];
+                f32x4 v = sums[wave * 256 + i * 64 + lane];
 #pragma unroll
-                for (int w = 1; w < kWaves; ++w)
-                    v += lds[(w * 4 + wave) * 256 + i * 64 + lane];
+                for (int u = 1; u < kWaves; ++u)
+                    v += sums[(u * VB + wave) * 256 + i * 64 + lane];
                 sum[nb][4 * i] = v[0], sum[nb][4 * i + 1] = v[1], sum[nb][4 * i + 2] = v[2], sum[nb][4 * i + 3] = v[3];
             }
         }
     }
     __syncthreads();  // the epilogue writes LDS
-    epilogue.template run<NB, OUT_ROWS>(o0, wave, lane, sum, reinterpret_cast<float *>(lds));
+    epilogue.template run<VB, NB, OUT_ROWS>(tile, nb0, a.blocks_n, wave, lane, sum, reinterpret_cast<float *>(lds));
 }
 
-// output (vocabulary entry, or feature) of element e of a lane's block m
-template <bool OUT_ROWS>
-__device__ inline int64_t output_of(int64_t o0, int m, int lane, int e)
+// place in the tile of element e of a lane's block m
+template <int VB, bool OUT_ROWS>
+__device__ inline int place_of(int m, int lane, int e)
 {
     const int r = 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-    return o0 + (OUT_ROWS ? 32 * m + r : 4 * r + m);
+    return OUT_ROWS ? 32 * m + r : VB * r + m;
 }
 
 struct RowsStatsEpilogue
 {
     const float *b;
     Labels labels;
-    int64_t V, n_pad;
+    int64_t V;
     float *part_m, *part_s, *target;
-    template <int NB, bool OUT_ROWS>
-    __device__ void run(int64_t o0, int m, int lane, f32x16 *z, float *lds) const
+    template <int VB, int NB, bool OUT_ROWS>
+    __device__ void run(int64_t tile, int nb0, int blocks_n, int m, int lane, f32x16 *z, float *lds) const
     {
-        float *lm = lds, *ls = lds + 4 * NB * 32;
-        if (m < 4)
+        float *lm = lds, *ls = lds + VB * NB * 32;
+        if (m < VB)
         {
+            float bias[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+            {
+                const int64_t v = tile * (32 * VB) + place_of<VB, OUT_ROWS>(m, lane, e);
+                bias[e] = v < V ? (b ? b[v] : 0.f) : -INFINITY;
+            }
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
             {
-                const int64_t n = nb * 32 + (lane & 31), label = labels(n);
+                const int64_t n = (nb0 + nb) * 32 + (lane & 31), label = labels(n) - tile * (32 * VB);
                 float top = -INFINITY;
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                 {
-                    const int64_t v = output_of<OUT_ROWS>(o0, m, lane, e);
-                    z[nb][e] = v < V ? z[nb][e] + (b ? b[v] : 0.f) : -INFINITY;
-                    if (v == label)
+                    // (past the vocabulary anything may have been read: selected away, not added to)
+                    z[nb][e] = bias[e] == -INFINITY ? -INFINITY : z[nb][e] + bias[e];
+                    if (place_of<VB, OUT_ROWS>(m, lane, e) == label)
                         target[n] = z[nb][e];
                     top = fmaxf(top, z[nb][e]);
                 }
@@ -234,74 +332,84 @@ struct RowsStatsEpilogue
             const int n = threadIdx.x;
             float m2 = lm[n], s = ls[n];
 #pragma unroll
-            for (int i = 1; i < 4; ++i)
+            for (int i = 1; i < VB; ++i)
                 merge(m2, s, lm[i * NB * 32 + n], ls[i * NB * 32 + n]);
-            part_m[(int64_t)blockIdx.x * n_pad + n] = m2, part_s[(int64_t)blockIdx.x * n_pad + n] = s;
+            const int64_t at = tile * (blocks_n * 32) + nb0 * 32 + n;
+            part_m[at] = m2, part_s[at] = s;
         }
     }
 };
 
-// d in the small operand's layout, dq[v / 4][rows][4], and gb
+// d split: by_n as the small operand of gx, [V / 16][blocks of 32 rows]; by_v as an operand of gw, rows of the vocabulary, [V / 32][rows
+// / 16] (null: not wanted); and the sums over this workgroup's rows for gb
 struct RowsGradEpilogue
 {
-    const float *b, *saved, *row, *gy;
+    const float *b, *saved, *row;
     Labels labels;
     int64_t V;
-    float *dq, *gb;
-    template <int NB, bool OUT_ROWS>
-    __device__ void run(int64_t o0, int m, int lane, f32x16 *z, float *) const
+    u32x4 *by_n, *by_v;
+    float *sums;  // [V padded to tiles][workgroups of rows]
+    template <int VB, int NB, bool OUT_ROWS>
+    __device__ void run(int64_t tile, int nb0, int blocks_n, int m, int lane, f32x16 *z, float *lds) const
     {
-        if (m >= 4)
-            return;
-        float sums[16];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
+        constexpr int kTile = 32 * VB, kPitch = 32 * NB + 1;
+        if (m < VB)
         {
-            const int64_t n = nb * 32 + (lane & 31), label = labels(n);
-            const bool counts = label >= 0;
-            const float m2 = counts ? row[2 * n] : 0.f, inv = counts ? 1.f / row[2 * n + 1] : 0.f;
+            float bias[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e)
             {
-                const int64_t v = output_of<OUT_ROWS>(o0, m, lane, e);
-                float d = 0.f;
-                if (counts && v < V)
-                {
-                    const float logit = z[nb][e] + (b ? b[v] : 0.f);
-                    d = pow2(fmaf(logit, kLog2e, -m2)) * inv;
-                    if (v == label)
-                        d -= 1.f;
-                }
-                z[nb][e] = d;
-                sums[e]  = nb ? sums[e] + d : d;
+                const int64_t v = tile * kTile + place_of<VB, OUT_ROWS>(m, lane, e);
+                bias[e] = v < V && b ? b[v] : 0.f;
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int nb = 0; nb < NB; ++nb)
             {
-                if constexpr (OUT_ROWS)
-                    *reinterpret_cast<f32x4 *>(dq + ((output_of<true>(o0, m, lane, 4 * i) / 4) * NB * 32 + n) * 4) =
-                        f32x4{z[nb][4 * i], z[nb][4 * i + 1], z[nb][4 * i + 2], z[nb][4 * i + 3]};
-                else
-                {
+                const int64_t n = (nb0 + nb) * 32 + (lane & 31), label = labels(n);
+                const bool counts = label >= 0;
+                const float m2 = counts ? row[2 * n] : 0.f, inv = counts ? 1.f / row[2 * n + 1] : 0.f;
 #pragma unroll
-                    for (int e = 4 * i; e < 4 * i + 4; ++e)
-                        dq[((output_of<false>(o0, m, lane, e) / 4) * NB * 32 + n) * 4 + m] = z[nb][e];
+                for (int e = 0; e < 16; ++e)
+                {
+                    const int at    = place_of<VB, OUT_ROWS>(m, lane, e);
+                    const int64_t v = tile * kTile + at;
+                    float d = 0.f;
+                    if (counts && v < V)
+                    {
+                        d = pow2(fmaf(z[nb][e] + bias[e], kLog2e, -m2)) * inv;
+                        if (v == label)
+                            d -= 1.f;
+                    }
+                    lds[at * kPitch + nb * 32 + (lane & 31)] = d;
                 }
             }
         }
-        if (!gb)
-            return;
-        const float g = (gy ? *gy : 1.f) / fmaxf(saved[kCounted], 1.f);
+        __syncthreads();
+        float v[8];
+        if (by_n)
+            for (int f = m; f < 2 * VB * NB; f += kWaves)
+            {
+                const int g = f / NB, nb = f % NB;
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
+                for (int e = 0; e < 8; ++e)
+                    v[e] = lds[(g * 16 + (lane >> 5) * 8 + e) * kPitch + nb * 32 + (lane & 31)];
+                store3(by_n + ((tile * (2 * VB) + g) * blocks_n + nb0 + nb) * kFragment, v, lane);
+            }
+        if (by_v)
+            for (int f = m; f < 2 * VB * NB; f += kWaves)
+            {
+                const int vb = f / (2 * NB), kb = f % (2 * NB);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    v[e] = lds[(vb * 32 + (lane & 31)) * kPitch + kb * 16 + (lane >> 5) * 8 + e];
+                store3(by_v + ((tile * VB + vb) * blocks_n * 2 + nb0 * 2 + kb) * kFragment, v, lane);
+            }
+        if (sums && threadIdx.x < kTile)
         {
-            float s = sums[e];
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1)
-                s += __shfl_xor(s, o, 64);
-            const int64_t v = output_of<OUT_ROWS>(o0, m, lane, e);
-            if ((lane & 31) == 0 && v < V)
-                gb[v] = s * g;
+            float s = 0.f;
+            for (int n = 0; n < 32 * NB; ++n)
+                s += lds[threadIdx.x * kPitch + n];
+            sums[(tile * kTile + threadIdx.x) * (blocks_n / NB) + nb0 / NB] = s;
         }
     }
 };
@@ -311,126 +419,145 @@ struct RowsPartEpilogue
 {
     float *parts;
     int64_t outs;
-    template <int NB, bool OUT_ROWS>
-    __device__ void run(int64_t o0, int m, int lane, f32x16 *z, float *) const
+    template <int VB, int NB, bool OUT_ROWS>
+    __device__ void run(int64_t tile, int nb0, int blocks_n, int m, int lane, f32x16 *z, float *) const
     {
-        if (m >= 4)
+        if (m >= VB)
             return;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
             {
-                const int64_t o = output_of<OUT_ROWS>(o0, m, lane, e);
+                const int64_t o = tile * (32 * VB) + place_of<VB, OUT_ROWS>(m, lane, e);
                 if (o < outs)
-                    parts[((int64_t)blockIdx.y * outs + o) * NB * 32 + nb * 32 + (lane & 31)] = z[nb][e];
+                    parts[((int64_t)blockIdx.y * outs + o) * (blocks_n * 32) + (nb0 + nb) * 32 + (lane & 31)] = z[nb][e];
             }
     }
 };
 
-// gx[n][k] = factor * the runs' sums, in order; a workgroup takes 32 features
+__global__ __launch_bounds__(kBlock) void ce_rows_gb_kernel(const float *__restrict__ sums, int groups, int64_t V, const float *saved, const float *gy, float *__restrict__ gb)
+{
+    const int64_t v = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (v >= V)
+        return;
+    float s = sums[v * groups];
+    for (int i = 1; i < groups; ++i)
+        s += sums[v * groups + i];
+    gb[v] = s * ((gy ? *gy : 1.f) / fmaxf(saved[kCounted], 1.f));
+}
+
+// gx[n][k] = factor * the runs' sums, in order; a workgroup takes 32 features and 32 rows
 __global__ __launch_bounds__(kBlock) void ce_rows_gx_kernel(const float *__restrict__ parts, int runs, int64_t N, int64_t K, int rows, const float *saved, const float *gy,
                                                             float *__restrict__ gx)
 {
-    __shared__ float tile[32][65];
+    __shared__ float tile[32][33];
     const float g = (gy ? *gy : 1.f) / fmaxf(saved[kCounted], 1.f);
-    const int64_t k0 = (int64_t)blockIdx.x * 32;
-    for (int i = threadIdx.x; i < 32 * rows; i += kBlock)
+    const int64_t k0 = (int64_t)blockIdx.x * 32, n0 = (int64_t)blockIdx.y * 32;
+    for (int i = threadIdx.x; i < 32 * 32; i += kBlock)
     {
-        const int k = i / rows, n = i % rows;
+        const int k = i / 32, n = i % 32;
         float s = 0.f;
         if (k0 + k < K)
 #pragma unroll 8
             for (int r = 0; r < runs; ++r)
-                s += parts[((int64_t)r * K + k0 + k) * rows + n];
+                s += parts[((int64_t)r * K + k0 + k) * rows + n0 + n];
         tile[k][n] = s * g;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < 32 * rows; i += kBlock)
+    for (int i = threadIdx.x; i < 32 * 32; i += kBlock)
     {
         const int n = i / 32, k = i % 32;
-        if (n < N && k0 + k < K)
-            gx[n * K + k0 + k] = tile[k][n];
+        if (n0 + n < N && k0 + k < K)
+            gx[(n0 + n) * K + k0 + k] = tile[k][n];
     }
 }
 
-// gw = factor * d^T.x over NB * 32 rows. out[r][c]: qc the operand of the stored rows' direction (16 bytes a lane: four columns),
-// qr the other one's. A wave keeps its 128 columns' operand in registers and walks down `steps` blocks of 32 rows.
-template <int NB>
-__global__ __launch_bounds__(kBlock) void ce_rows_outer_kernel(const f32x4 *__restrict__ qc, const float *__restrict__ qr, int64_t rows, int64_t cols, unsigned tiles_c, int steps,
-                                                               const float *saved, const float *gy, float *__restrict__ out)
+// gw = factor * d^T.x over the rows: out[r][c] from operands split by r and by c, [blocks of 32][rows / 16]. A wave makes 32 rows of 128
+// columns; the four waves of a workgroup share the columns' operand, and walk down `steps` blocks of 128 rows.
+__global__ __launch_bounds__(kBlock, 2) void ce_rows_outer_kernel(const u32x4 *__restrict__ by_r, const u32x4 *__restrict__ by_c, int kbs, int64_t rows, int64_t cols,
+                                                                  unsigned tiles_c, int steps, const float *saved, const float *gy, float *__restrict__ out)
 {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5, i32 = lane & 31;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const float g = (gy ? *gy : 1.f) / fmaxf(saved[kCounted], 1.f);
     const unsigned group = blockIdx.x / tiles_c;
     const int64_t c0 = (int64_t)(blockIdx.x - group * tiles_c) * 128;
-    f32x4 c[NB * 16];
-#pragma unroll
-    for (int i = 0; i < NB * 16; ++i)
-        c[i] = qc[(c0 / 4 + i32) * NB * 32 + 2 * i + half];
-    const int64_t col = c0 + i32 * 4;
     for (int step = 0; step < steps; ++step)
     {
         const int64_t r0 = (((int64_t)group * steps + step) * 4 + wave) * 32;
         if (r0 >= rows)
             return;
-        const float *q = qr + ((r0 + i32) / 4) * NB * 32 * 4 + (i32 & 3);
+        const u32x4 *r = by_r + r0 / 32 * kbs * kFragment + lane, *c = by_c + c0 / 32 * kbs * kFragment + lane;
         f32x16 acc[4];
 #pragma unroll
         for (int m = 0; m < 4; ++m)
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 acc[m][e] = 0.f;
-        float r[NB * 16];
+#pragma unroll 2
+        for (int kb = 0; kb < kbs; ++kb)
+        {
+            u32x4 a[3], b[4][3];
 #pragma unroll
-        for (int i = 0; i < NB * 16; ++i)
-            r[i] = q[(2 * i + half) * 4];
-#pragma unroll
-        for (int i = 0; i < NB * 16; ++i)
+            for (int p = 0; p < 3; ++p)
+                a[p] = r[kb * kFragment + p * 64];
 #pragma unroll
             for (int m = 0; m < 4; ++m)
-                acc[m] = __builtin_amdgcn_mfma_f32_32x32x2f32(r[i], c[i][m], acc[m], 0, 0, 0);
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
+                for (int p = 0; p < 3; ++p)
+                    b[m][p] = c[(m * kbs + kb) * kFragment + p * 64];
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+                multiply(acc[m], a, b[m]);
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m)
         {
-            const int64_t row = r0 + 8 * (e >> 2) + 4 * half + (e & 3);
-            if (row >= rows)
+            const int64_t col = c0 + m * 32 + (lane & 31);
+            if (col >= cols)
                 continue;
-            float *at = out + row * cols + col;
-            if (col + 3 < cols)
-                *reinterpret_cast<f32x4u *>(at) = f32x4{acc[0][e] * g, acc[1][e] * g, acc[2][e] * g, acc[3][e] * g};
-            else
-            {
 #pragma unroll
-                for (int m = 0; m < 4; ++m)
-                    if (col + m < cols)
-                        at[m] = acc[m][e] * g;
+            for (int e = 0; e < 16; ++e)
+            {
+                const int64_t row = r0 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+                if (row < rows)
+                    out[row * cols + col] = acc[m][e] * g;
             }
         }
     }
 }
 
-int rows_of(int64_t N)
+// blocks of 32 rows that a call's rows take, and how many a workgroup of a stream has: 1, 2 or 4
+int blocks_of(int64_t N)
 {
-    return N <= 32 ? 32 : 64;
+    return N <= 32 ? 1 : N <= 64 ? 2 : N <= 128 ? 4 : 8;
+}
+int taken_of(int blocks_n)
+{
+    return std::min(blocks_n, 4);
+}
+// outputs of a stream's workgroup: accumulators of 128 x 64 or 64 x 128
+int64_t tile_of(int blocks_n)
+{
+    return taken_of(blocks_n) == 4 ? 64 : 128;
 }
 
-// quads of a small operand: whole tiles of 128, so that a tile of gw reads only what exists
-int64_t quads_of(int64_t n)
+// fragments of an operand with `rows` rows: whole tiles of 128, so that what a stream or a tile of gw reaches is there
+size_t fragments_bytes(int64_t rows, int64_t blocks_n)
 {
-    return odl::ceil_div(n, 128) * 32;
+    return (size_t)odl::ceil_div(rows, 128) * 8 * (size_t)blocks_n * kFragment * 16;
 }
 
-int runs_for_gx(int64_t K, int64_t V)
+int runs_for_gx(int64_t K, int64_t V, int blocks_n)
 {
-    const int64_t tiles = odl::ceil_div(K, kTile);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(odl::device_cus() / tiles, odl::ceil_div(V, 128)));
+    const int64_t groups = odl::ceil_div(K, tile_of(blocks_n)) * (blocks_n / taken_of(blocks_n));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(odl::device_cus() / groups, odl::ceil_div(V, 256)));
 }
 
 struct FewSpace
 {
-    f32x4 *xq;
-    float *part_m, *part_s, *target, *dq, *parts;
+    u32x4 *x_by_n, *x_by_k, *d_by_n, *d_by_v;
+    float *part_m, *part_s, *target, *parts, *sums;
     void *join_scratch;
     size_t bytes;
 };
@@ -439,8 +566,9 @@ FewSpace forward_space(char *base, int64_t N, int64_t K, int64_t V)
 {
     FewSpace s{};
     Carver c{base};
-    const size_t rows = (size_t)rows_of(N), tiles = (size_t)odl::ceil_div(V, kTile);
-    s.xq           = c.take<f32x4>((size_t)quads_of(K) * rows * 16);
+    const int blocks_n = blocks_of(N);
+    const size_t rows = (size_t)blocks_n * 32, tiles = (size_t)odl::ceil_div(V, tile_of(blocks_n));
+    s.x_by_n       = c.take<u32x4>(fragments_bytes(K, blocks_n));
     s.part_m       = c.take<float>(tiles * rows * 4);
     s.part_s       = c.take<float>(tiles * rows * 4);
     s.target       = c.take<float>(rows * 4);
@@ -453,36 +581,44 @@ FewSpace backward_space(char *base, int64_t N, int64_t K, int64_t V)
 {
     FewSpace s{};
     Carver c{base};
-    const size_t rows = (size_t)rows_of(N);
-    s.xq    = c.take<f32x4>((size_t)quads_of(K) * rows * 16);
-    s.dq    = c.take<float>((size_t)quads_of(V) * rows * 16);
-    s.parts = c.take<float>((size_t)runs_for_gx(K, V) * (size_t)K * rows * 4);
-    s.bytes = c.used;
+    const int blocks_n = blocks_of(N);
+    s.x_by_n = c.take<u32x4>(fragments_bytes(K, blocks_n));
+    s.x_by_k = c.take<u32x4>(fragments_bytes(K, blocks_n));
+    s.d_by_n = c.take<u32x4>(fragments_bytes(V, blocks_n));
+    s.d_by_v = c.take<u32x4>(fragments_bytes(V, blocks_n));
+    s.sums   = c.take<float>((size_t)odl::ceil_div(V, 128) * 128 * 2 * 4);
+    s.parts  = c.take<float>((size_t)runs_for_gx(K, V, blocks_n) * (size_t)K * (size_t)blocks_n * 32 * 4);
+    s.bytes  = c.used;
     return s;
 }
 
 template <class Epilogue>
-int stream(const float *w, bool out_rows, int64_t ld, int64_t outs, int64_t contraction, const void *q, int rows, int runs, const Epilogue &e, hipStream_t st)
+int stream(const float *w, bool out_rows, int64_t ld, int64_t outs, int64_t contraction, const u32x4 *q, int blocks_n, int runs, const Epilogue &e, hipStream_t st)
 {
-    Stream a{w, ld, outs, contraction, static_cast<const f32x4 *>(q), odl::ceil_div(contraction, 8), 0};
+    Stream a{w, ld, outs, contraction, q, blocks_n, odl::ceil_div(contraction, 16), 0};
     a.wave_groups = odl::ceil_div(a.groups, (int64_t)runs * kWaves);
-    const dim3 grid((unsigned)odl::ceil_div(outs, kTile), (unsigned)runs), block(64 * kWaves);
-    if (rows == 32 && out_rows)
-        ce_stream_kernel<1, true, Epilogue><<<grid, block, 0, st>>>(a, e);
-    else if (rows == 32)
-        ce_stream_kernel<1, false, Epilogue><<<grid, block, 0, st>>>(a, e);
-    else if (out_rows)
-        ce_stream_kernel<2, true, Epilogue><<<grid, block, 0, st>>>(a, e);
-    else
-        ce_stream_kernel<2, false, Epilogue><<<grid, block, 0, st>>>(a, e);
+    const int64_t blocks = odl::ceil_div(outs, tile_of(blocks_n)) * (blocks_n / taken_of(blocks_n));
+    ODL_REQUIRE(blocks < ((int64_t)1 << 31), "linear_softmax_ce: too many tiles");
+    const dim3 grid((unsigned)blocks, (unsigned)runs), block(64 * kWaves);
+    switch (taken_of(blocks_n) * 2 + (out_rows ? 1 : 0))
+    {
+        case 2: ce_stream_kernel<4, 1, false, Epilogue><<<grid, block, 0, st>>>(a, e); break;
+        case 3: ce_stream_kernel<4, 1, true, Epilogue><<<grid, block, 0, st>>>(a, e); break;
+        case 4: ce_stream_kernel<4, 2, false, Epilogue><<<grid, block, 0, st>>>(a, e); break;
+        case 5: ce_stream_kernel<4, 2, true, Epilogue><<<grid, block, 0, st>>>(a, e); break;
+        case 8: ce_stream_kernel<2, 4, false, Epilogue><<<grid, block, 0, st>>>(a, e); break;
+        default: ce_stream_kernel<2, 4, true, Epilogue><<<grid, block, 0, st>>>(a, e); break;
+    }
     ODL_LAUNCH_CHECK();
     return ODL_OK;
 }
 
-int prepare(const Problem &p, int rows, f32x4 *xq, float *saved, hipStream_t st)
+// whole tiles of 128 features: a tile of gw reads them all
+int prepare(const Problem &p, int blocks_n, u32x4 *by_n, u32x4 *by_k, float *saved, hipStream_t st)
 {
-    const int64_t quads = quads_of(p.K);
-    ce_rows_prepare_kernel<<<dim3((unsigned)odl::ceil_div(quads * rows, kBlock)), dim3(kBlock), 0, st>>>(p.x, p.K, p.labels, rows, quads, xq, saved);
+    const int64_t groups = odl::ceil_div(p.K, 128) * 8, blocks_k = groups / 2;
+    ce_rows_prepare_kernel<<<dim3((unsigned)odl::ceil_div(groups * blocks_n, kBlock / 64)), dim3(kBlock), 0, st>>>(p.x, p.K, p.labels, blocks_n, groups, blocks_k,
+                                                                                                            by_n, by_k, saved);
     ODL_LAUNCH_CHECK();
     return ODL_OK;
 }
@@ -504,49 +640,50 @@ size_t few_backward_bytes(int64_t N, int64_t K, int64_t V)
 
 int few_forward(const Problem &p, float *saved, float *row_stats, char *workspace, hipStream_t st)
 {
-    const int rows = rows_of(p.N);
-    const FewSpace s = ::forward_space(workspace, p.N, p.K, p.V);
-    if (int rc = prepare(p, rows, s.xq, saved, st))
+    const int blocks_n = blocks_of(p.N);
+    const FewSpace s   = ::forward_space(workspace, p.N, p.K, p.V);
+    if (int rc = prepare(p, blocks_n, s.x_by_n, nullptr, saved, st))
         return rc;
-    const RowsStatsEpilogue e{p.b, p.labels, p.V, rows, s.part_m, s.part_s, s.target};
-    if (int rc = stream(p.w, p.w_out_in != 0, p.w_out_in ? p.K : p.V, p.V, p.K, s.xq, rows, 1, e, st))
+    const RowsStatsEpilogue e{p.b, p.labels, p.V, s.part_m, s.part_s, s.target};
+    if (int rc = stream(p.w, p.w_out_in != 0, p.w_out_in ? p.K : p.V, p.V, p.K, s.x_by_n, blocks_n, 1, e, st))
         return rc;
-    return join(s.part_m, s.part_s, s.target, ceil_div(p.V, kTile), rows, p.labels, row_stats, s.join_scratch, saved, st);
+    return join(s.part_m, s.part_s, s.target, ceil_div(p.V, tile_of(blocks_n)), blocks_n * 32, p.labels, row_stats, s.join_scratch, saved, st);
 }
 
 int few_backward(const Problem &p, const float *gy, const float *saved, const float *row_stats, float *gx, float *gw, float *gb, char *workspace,
                  hipStream_t st)
 {
-    const int rows = rows_of(p.N);
-    const FewSpace s = ::backward_space(workspace, p.N, p.K, p.V);
-    if (int rc = prepare(p, rows, s.xq, nullptr, st))
+    const int blocks_n = blocks_of(p.N);
+    const FewSpace s   = ::backward_space(workspace, p.N, p.K, p.V);
+    if (int rc = prepare(p, blocks_n, s.x_by_n, gw ? s.x_by_k : nullptr, nullptr, st))
         return rc;
     const int64_t ld = p.w_out_in ? p.K : p.V;
-    const RowsGradEpilogue e{p.b, saved, row_stats, gy, p.labels, p.V, s.dq, gb};
-    if (int rc = stream(p.w, p.w_out_in != 0, ld, p.V, p.K, s.xq, rows, 1, e, st))
+    const RowsGradEpilogue e{p.b, saved, row_stats, p.labels, p.V, gx ? s.d_by_n : nullptr, gw ? s.d_by_v : nullptr, gb ? s.sums : nullptr};
+    if (int rc = stream(p.w, p.w_out_in != 0, ld, p.V, p.K, s.x_by_n, blocks_n, 1, e, st))
         return rc;
+    if (gb)
+    {
+        ce_rows_gb_kernel<<<dim3((unsigned)ceil_div(p.V, kBlock)), dim3(kBlock), 0, st>>>(s.sums, blocks_n / taken_of(blocks_n), p.V, saved, gy, gb);
+        ODL_LAUNCH_CHECK();
+    }
     if (gx)
     {
-        const int runs = runs_for_gx(p.K, p.V);
-        if (int rc = stream(p.w, p.w_out_in == 0, ld, p.K, p.V, s.dq, rows, runs, RowsPartEpilogue{s.parts, p.K}, st))
+        const int runs = runs_for_gx(p.K, p.V, blocks_n);
+        if (int rc = stream(p.w, p.w_out_in == 0, ld, p.K, p.V, s.d_by_n, blocks_n, runs, RowsPartEpilogue{s.parts, p.K}, st))
             return rc;
-        ce_rows_gx_kernel<<<dim3((unsigned)ceil_div(p.K, 32)), dim3(kBlock), 0, st>>>(s.parts, runs, p.N, p.K, rows, saved, gy, gx);
+        ce_rows_gx_kernel<<<dim3((unsigned)ceil_div(p.K, 32), (unsigned)blocks_n), dim3(kBlock), 0, st>>>(s.parts, runs, p.N, p.K, blocks_n * 32, saved, gy, gx);
         ODL_LAUNCH_CHECK();
     }
     if (gw)
     {
         const int64_t r = p.w_out_in ? p.V : p.K, c = p.w_out_in ? p.K : p.V;
-        const void *qc = p.w_out_in ? (const void *)s.xq : s.dq, *qr = p.w_out_in ? (const void *)s.dq : s.xq;
-        // enough workgroups for the chip, and as many rows each as that leaves: the columns' operand is read once per workgroup
+        // enough workgroups for the chip, and as many rows each as that leaves: they share the columns' operand
         const int64_t tiles_c = ceil_div(c, 128), tiles_r = ceil_div(r, 128);
         const int steps = (int)std::max<int64_t>(1, std::min<int64_t>(16, tiles_c * tiles_r / (8 * (int64_t)device_cus())));
         const int64_t blocks = tiles_c * ceil_div(tiles_r, steps);
-        ODL_REQUIRE(blocks < ((int64_t)1 << 31), "weight gradient of too many tiles");
-        const dim3 grid((unsigned)blocks);
-        if (rows == 32)
-            ce_rows_outer_kernel<1><<<grid, dim3(kBlock), 0, st>>>(static_cast<const f32x4 *>(qc), static_cast<const float *>(qr), r, c, (unsigned)tiles_c, steps, saved, gy, gw);
-        else
-            ce_rows_outer_kernel<2><<<grid, dim3(kBlock), 0, st>>>(static_cast<const f32x4 *>(qc), static_cast<const float *>(qr), r, c, (unsigned)tiles_c, steps, saved, gy, gw);
+        ODL_REQUIRE(blocks < ((int64_t)1 << 31), "linear_softmax_ce: too many tiles");
+        ce_rows_outer_kernel<<<dim3((unsigned)blocks), dim3(kBlock), 0, st>>>(p.w_out_in ? s.d_by_v : s.x_by_k, p.w_out_in ? s.x_by_k : s.d_by_v, blocks_n * 2, r, c,
+                                                                             (unsigned)tiles_c, steps, saved, gy, gw);
         ODL_LAUNCH_CHECK();
     }
     return ODL_OK;

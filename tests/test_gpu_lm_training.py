@@ -90,8 +90,9 @@ def check(got, want, bars):
 # one token to many, one feature, one class, sizes around every tile (64, 128, 256) and its half, and several pieces
 CE_SHAPES = [(1, 1, 1), (1, 64, 1000), (2, 3, 5), (3, 17, 64), (5, 33, 65), (16, 100, 130), (31, 257, 511), (64, 128, 256), (65, 96, 97),
              (96, 769, 300), (128, 64, 1025), (200, 768, 2000), (257, 130, 769), (770, 100, 3001), (1025, 300, 1100), (33, 40, 129), (1, 4097, 3), (8, 5, 6000),
-             # few rows over large weights stream them: ends of the vocabulary and of K off every step, 32 rows and 64
-             (1, 64, 100000), (7, 129, 50003), (32, 2050, 3001), (33, 2047, 3002), (64, 100, 60004), (5, 1000003, 6), (64, 2000, 4001)]
+             # few rows over large weights stream them: ends of the vocabulary and of K off every step, 32 rows to 256
+             (1, 64, 100000), (7, 129, 50003), (32, 2050, 3001), (33, 2047, 3002), (64, 100, 60004), (5, 1000003, 6), (64, 2000, 4001), (65, 300, 30001), (128, 1031, 6002),
+             (129, 64, 100003), (200, 2000, 3500), (256, 515, 12007)]
 
 
 @pytest.mark.parametrize("shape", CE_SHAPES)
