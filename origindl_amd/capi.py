@@ -10,6 +10,7 @@ broadcast_to, max, softmax, gather, one_hot, softmax_cross_entropy(+_backward), 
 accuracy, and the elementwise set. Errors surface as OdlInvalidArgument / OdlRuntimeError, the counterparts of
 the reference's std::invalid_argument / std::runtime_error."""
 import builtins as _builtins
+import contextlib as _contextlib
 import ctypes
 
 import numpy as np
@@ -487,6 +488,19 @@ def softmax_cross_entropy_with_unit_grad(x, t):
     return float(words[0]), int(words.view(torch.int32)[1]), gx
 
 
+_NO_GUARD = _contextlib.nullcontext()
+
+
+def _on(device):
+    """Makes `device` current for the calls inside, where it is not already."""
+    return _NO_GUARD if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _ws_like(x, nbytes):
+    """A workspace on x's device."""
+    return (x.new_empty(nbytes, dtype=torch.uint8), nbytes) if nbytes else (None, 0)
+
+
 # ------------------------------------------------------ output layer with its loss, large vocabularies
 def _ce_args(who, x, w, b, t, w_out_in):
     _chk(x, "x"), _chk(w, "w")
@@ -512,9 +526,9 @@ def linear_softmax_cross_entropy(x, w, b, t, ignore_index=-100, w_out_in=False):
     saved = (words, row_stats) for the backward pass; words[1] viewed as int32 is nonzero after a label out of range (see
     linear_softmax_cross_entropy_bad_label). w: [K, V], or [V, K] with w_out_in. Does not synchronise."""
     N, K, V, is64 = _ce_args("linear_softmax_cross_entropy", x, w, b, t, w_out_in)
-    with torch.cuda.device(x.device):
-        saved, rows = _empty((8,)), _empty((N, 2))
-        ws, nb = _ws(lib().query("odl_hip_linear_softmax_ce_forward_workspace_bytes", N, K, V))
+    with _on(x.device):
+        saved, rows = x.new_empty(8), x.new_empty((N, 2))
+        ws, nb = _ws_like(x, lib().query("odl_hip_linear_softmax_ce_forward_workspace_bytes", N, K, V))
         lib().call("odl_hip_linear_softmax_ce_forward", _p(x), _p(w), int(w_out_in), _p(b), _p(t), is64, int(ignore_index), N, K, V,
                    _p(saved), _p(rows), _p(ws), nb, _stream())
     return saved[0], (saved, rows)
@@ -534,11 +548,11 @@ def linear_softmax_cross_entropy_backward(gy, x, w, b, t, saved, ignore_index=-1
     words, rows = _chk(saved[0], "saved"), _chk(saved[1], "saved")
     if words.numel() != 8 or tuple(rows.shape) != (N, 2) or words.device != x.device or rows.device != x.device:
         raise OdlInvalidArgument("linear_softmax_cross_entropy_backward: saved is not from a forward call with %d rows" % N)
-    with torch.cuda.device(x.device):
-        gx = _empty((N, K)) if need_gx else None
-        gw = _empty(w.shape) if need_gw else None
-        gb = _empty((V,)) if need_gb else None
-        ws, nb = _ws(lib().query("odl_hip_linear_softmax_ce_backward_workspace_bytes", N, K, V))
+    with _on(x.device):
+        gx = x.new_empty((N, K)) if need_gx else None
+        gw = torch.empty_like(w) if need_gw else None
+        gb = x.new_empty(V) if need_gb else None
+        ws, nb = _ws_like(x, lib().query("odl_hip_linear_softmax_ce_backward_workspace_bytes", N, K, V))
         lib().call("odl_hip_linear_softmax_ce_backward", _p(gy), _p(x), _p(w), int(w_out_in), _p(b), _p(t), is64, int(ignore_index), N, K,
                    V, _p(words), _p(rows), _p(gx), _p(gw), _p(gb), _p(ws), nb, _stream())
     return gx, gw, gb
@@ -1125,9 +1139,9 @@ def newton_schulz(g, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
         raise OdlInvalidArgument("newton_schulz: g must be 2D or 3D, got %s" % (tuple(g.shape),))
     batch, rows, cols = (1,) + tuple(g.shape) if g.dim() == 2 else tuple(g.shape)
     a, b, c = (float(v) for v in coefficients)
-    with torch.cuda.device(g.device):
-        out = _empty(g.shape)
-        ws, nb = _ws(lib().query("odl_hip_newton_schulz_workspace_bytes", batch, rows, cols))
+    with _on(g.device):
+        out = torch.empty_like(g)
+        ws, nb = _ws_like(g, lib().query("odl_hip_newton_schulz_workspace_bytes", batch, rows, cols))
         lib().call("odl_hip_newton_schulz", _p(g), batch, rows, cols, int(steps), a, b, c, float(eps), _p(out), _p(ws), nb, _stream())
     return out
 
@@ -1138,21 +1152,25 @@ def muon_step_multi(ps, gs, bufs, lr, momentum=0.95, nesterov=True, weight_decay
     parameters p * (1 - lr * weight_decay) - lr * sqrt(max(1, rows / cols)) * newton_schulz(update)."""
     if not (len(ps) == len(gs) == len(bufs)):
         raise OdlInvalidArgument("muon_step_multi: lists of different lengths")
-    for p, g, buf in zip(ps, gs, bufs):
-        for x in (p, g, buf):
-            if _chk(x, "muon_step_multi operand").dim() != 2 or x.shape != p.shape or x.device != ps[0].device:
-                raise OdlInvalidArgument("muon_step_multi: parameter, gradient and buffer must be matrices of one shape on one device")
-    if len({buf.data_ptr() for buf in bufs if buf.numel()}) != _builtins.sum(1 for buf in bufs if buf.numel()):
-        raise OdlInvalidArgument("muon_step_multi: a buffer stands for two entries")
     if not ps:
         return []
-    n = len(ps)
-    rows = (ctypes.c_int64 * n)(*[int(p.shape[0]) for p in ps])
-    cols = (ctypes.c_int64 * n)(*[int(p.shape[1]) for p in ps])
+    n, device = len(ps), ps[0].device
+    rows, cols, kept = (ctypes.c_int64 * n)(), (ctypes.c_int64 * n)(), set()
+    for i in range(n):
+        p, g, buf = ps[i], gs[i], bufs[i]
+        shape = p.shape
+        for x in (p, g, buf):
+            if _chk(x, "muon_step_multi operand").shape != shape or len(shape) != 2 or x.device != device:
+                raise OdlInvalidArgument("muon_step_multi: parameter, gradient and buffer must be matrices of one shape on one device")
+        rows[i], cols[i] = shape
+        at = buf.data_ptr()
+        if at and at in kept:
+            raise OdlInvalidArgument("muon_step_multi: a buffer stands for two entries")
+        kept.add(at)
     a, b, c = (float(v) for v in coefficients)
-    with torch.cuda.device(ps[0].device):
-        outs = [_empty(p.shape) for p in ps]
-        ws, nb = _ws(lib().query("odl_hip_muon_step_multi_workspace_bytes", n, rows, cols))
+    with _on(device):
+        outs = [torch.empty_like(p) for p in ps]
+        ws, nb = _ws_like(ps[0], lib().query("odl_hip_muon_step_multi_workspace_bytes", n, rows, cols))
         lib().call("odl_hip_muon_step_multi", n, _ptr_array(ps), _ptr_array(gs), _ptr_array(bufs), rows, cols, float(lr), float(momentum),
                    int(nesterov), float(weight_decay), int(steps), a, b, c, float(eps), _ptr_array(outs), _p(ws), nb, _stream())
     return outs
