@@ -406,9 +406,22 @@ struct RowsGradEpilogue
             }
         if (sums && threadIdx.x < kTile)
         {
-            float s = 0.f;
-            for (int n = 0; n < 32 * NB; ++n)
-                s += lds[threadIdx.x * kPitch + n];
+            // sixteen sums and a tree over them: a long chain would round every time
+            float part[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                part[i] = lds[threadIdx.x * kPitch + i];
+            for (int n = 16; n < 32 * NB; n += 16)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    part[i] += lds[threadIdx.x * kPitch + n + i];
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < o)
+                        part[i] += part[i + o];
+            const float s = part[0];
             sums[(tile * kTile + threadIdx.x) * (blocks_n / NB) + nb0 / NB] = s;
         }
     }

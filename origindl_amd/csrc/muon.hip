@@ -14,7 +14,6 @@
 // Singular values of X stay under max |f| on [0, 1], f(s) = a s + b s^3 + c s^5 (1.21 for the usual coefficients), so all
 // operands are scaled by the same 2^13: float16 holds 8 * 2^13, and coefficients that lead past 7.5 are refused.
 #include <cmath>
-#include <vector>
 
 #include "muon.h"
 
@@ -365,11 +364,13 @@ extern "C" int odl_hip_muon_step_multi(int count, const float *const *p, const f
                 workspace ? workspace_bytes : (size_t)0);
     ODL_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 15) == 0, "%s: the workspace must be 16-byte aligned", who);
     ODL_REQUIRE_DEVICE();
-    std::vector<char> done((size_t)count, 0);
     for (int i = 0; i < count; ++i)
     {
         const int64_t rows = host_rows[i], cols = host_cols[i];
-        if (done[(size_t)i] || rows == 0 || cols == 0)
+        bool done = rows == 0 || cols == 0;
+        for (int j = 0; j < i && !done; ++j)
+            done = host_rows[j] == rows && host_cols[j] == cols;
+        if (done)
             continue;
         // all entries of this shape, a group at a time
         int equal = 0;
@@ -384,7 +385,6 @@ extern "C" int odl_hip_muon_step_multi(int count, const float *const *p, const f
         {
             if (host_rows[j] != rows || host_cols[j] != cols)
                 continue;
-            done[(size_t)j] = 1;
             mat.g[in] = g[j], mat.buf[in] = buf[j], mat.p[in] = p[j], mat.out[in] = p_out[j], ++in, --equal;
             if (in == group || equal == 0)
             {
