@@ -5,7 +5,7 @@
 // five. So a workgroup takes a strip of the long side, all m rows of it, and does a whole step: it adds up the strips' shares
 // of A = X X^T, forms b A + c A A in LDS (every workgroup for itself: m^3 operations), multiplies it with its strip of X, and
 // leaves its strip's share of the next A. Operands are those of split_gemm.h; A and b A + c A A never leave LDS, X's strip is
-// updated in place (nobody else reads it), the shares alternate between two places.
+// updated in place (nobody else reads it), the shares alternate between two places. A matrix of one strip stays in LDS whole.
 //
 // A matrix of one strip needs no other workgroup: momentum, norm and all steps are one launch.
 //
@@ -81,6 +81,29 @@ __device__ inline void multiply_blocks(f32x16 *acc, const Panel &a, int64_t ra, 
     }
 }
 
+// store_mirror through half the scratch, sixteen rows at a time
+__device__ inline void store_mirror_halves(const Panel &p, int64_t rb, int64_t cb, int lane, const f32x16 &c, float *scratch)
+{
+    float v[2][8];
+#pragma unroll
+    for (int part = 0; part < 2; ++part)
+    {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            scratch[(8 * (lane >> 5) + e) * 33 + (lane & 31)] = c[8 * part + e];
+        __builtin_amdgcn_wave_barrier();
+        if (((lane & 31) >> 4) == part)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    v[h][e] = scratch[(lane & 15) * 33 + 16 * h + 8 * (lane >> 5) + e];
+        __builtin_amdgcn_wave_barrier();
+    }
+    store_fragment(p, rb, cb * 2, lane, v[0]);
+    store_fragment(p, rb, cb * 2 + 1, lane, v[1]);
+}
+
 __device__ inline void clear(f32x16 &c)
 {
 #pragma unroll
@@ -98,27 +121,29 @@ __global__ __launch_bounds__(MB == 4 ? 512 : 256, 2) void muon_slim_kernel(const
     constexpr int kScratch = W * 32 * 33 * 4, kTileF = M * (C + 1) * 4;
     constexpr int kFirstRegion = kSquare > kScratch ? kSquare : kScratch, kLarger = kSquare > kStrip ? kSquare : kStrip;
     constexpr int kSecond = kLarger > kScratch ? kLarger : kScratch;
-    constexpr int kLds = kFirstRegion + kSecond > kTileF + kStrip ? kFirstRegion + kSecond : kTileF + kStrip;
+    // one strip: X by columns, then what is needed in turn — X by rows, A, b A + c A A —, then half the scratch
+    constexpr int kWholeLds = kStrip + (kTileF > kLarger + kScratch / 2 ? kTileF : kLarger + kScratch / 2);
+    constexpr int kLds = MODE == kWhole ? kWholeLds : kFirstRegion + kSecond > kTileF + kStrip ? kFirstRegion + kSecond : kTileF + kStrip;
     __shared__ __attribute__((aligned(16))) char lds[kLds];
     __shared__ double norm_parts[W];
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
     const int strip = blockIdx.x, z = blockIdx.y;
-    const Panel xt{s.xt + z * s.xt_bytes, MB * 2};
+    const Panel xt{MODE == kWhole ? lds : s.xt + z * s.xt_bytes, MB * 2};
     const int64_t rb0 = (int64_t)strip * CB;  // the strip's first row block in xt
-    float *scratch = reinterpret_cast<float *>(lds) + wave * (32 * 33);
+    float *scratch = MODE == kWhole ? reinterpret_cast<float *>(lds + kStrip + kLarger) + wave * (16 * 33) : reinterpret_cast<float *>(lds) + wave * (32 * 33);
     Panel rows{nullptr, CB * 2};  // the strip as rows of m, for its share of A
 
     if constexpr (MODE == kFirst || MODE == kWhole)
     {
-        rows.base  = lds + kTileF;
-        float *tile = reinterpret_cast<float *>(lds);  // [m][C + 1]
+        rows.base  = lds + (MODE == kWhole ? kStrip : kTileF);
+        float *tile = reinterpret_cast<float *>(lds + (MODE == kWhole ? kStrip : 0));  // [m][C + 1]
         double factor = 1.0, squares = 0.0;
         if constexpr (MODE == kFirst)
             factor = (double)kScale / (sqrt(sum_of_parts<W>(s.sums + (int64_t)z * s.parts, s.parts, norm_parts)) + s.eps);
         const Update u{s.a.g[z], s.a.buf[z], s.a.momentum, s.a.nesterov};
         const bool tall = s.a.rows > s.a.cols;
         const int64_t m = tall ? s.a.cols : s.a.rows, n = tall ? s.a.rows : s.a.cols, n0 = (int64_t)strip * C;
-#pragma unroll 8
+#pragma unroll 16
         for (int i = threadIdx.x; i < M * C; i += W * 64)
         {
             // lanes along what lies contiguous
@@ -167,19 +192,27 @@ __global__ __launch_bounds__(MB == 4 ? 512 : 256, 2) void muon_slim_kernel(const
                 v[e] = (float)((double)tile[(kb * 16 + (lane >> 5) * 8 + e) * (C + 1) + cb * 32 + (lane & 31)] * factor);
             store_fragment(xt, rb0 + cb, kb, lane, v);
         }
-        for (int f = wave; f < MB * CB * 2; f += W)
+        float v[MB * CB * 2 / W][8];
+#pragma unroll
+        for (int i = 0; i < MB * CB * 2 / W; ++i)
         {
-            const int rb = f / (CB * 2), kb = f % (CB * 2);
-            float v[8];
+            const int f = wave + i * W, rb = f / (CB * 2), kb = f % (CB * 2);
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                v[e] = (float)((double)tile[(rb * 32 + (lane & 31)) * (C + 1) + kb * 16 + (lane >> 5) * 8 + e] * factor);
-            store_fragment(rows, rb, kb, lane, v);
+                v[i][e] = (float)((double)tile[(rb * 32 + (lane & 31)) * (C + 1) + kb * 16 + (lane >> 5) * 8 + e] * factor);
+        }
+        if constexpr (MODE == kWhole)
+            __syncthreads();  // the rows go where the values came from
+#pragma unroll
+        for (int i = 0; i < MB * CB * 2 / W; ++i)
+        {
+            const int f = wave + i * W, rb = f / (CB * 2), kb = f % (CB * 2);
+            store_fragment(rows, rb, kb, lane, v[i]);
         }
     }
     constexpr int PP = (kPairs + W - 1) / W;
     constexpr int kSquareBlocks = MB * MB / W, kStripBlocks = MB * CB / W;  // a wave's: one row block of m, neighbouring columns
-    const Panel square{lds, MB * 2}, poly{lds + kFirstRegion, MB * 2};
+    const Panel square{lds + (MODE == kWhole ? kStrip : 0), MB * 2}, poly{lds + (MODE == kWhole ? kStrip : kFirstRegion), MB * 2};
     if constexpr (MODE == kWhole)
         __syncthreads();
     for (int k = 1;; ++k)
@@ -193,7 +226,7 @@ __global__ __launch_bounds__(MB == 4 ? 512 : 256, 2) void muon_slim_kernel(const
                 for (f32x16 &c : a)
                     clear(c);
                 multiply_blocks<kSquareBlocks>(a, rows, wave % MB, rows, wave / MB * kSquareBlocks, CB * 2, lane);
-                __syncthreads();  // the first strip's rows may lie where A goes
+                __syncthreads();  // A goes where the rows lie
 #pragma unroll
                 for (int i = 0; i < kSquareBlocks; ++i)
                 {
@@ -247,8 +280,12 @@ __global__ __launch_bounds__(MB == 4 ? 512 : 256, 2) void muon_slim_kernel(const
                 const int bj = wave / MB * kSquareBlocks + i;
                 to_columns(b[i]);
                 combine(b[i], square, bj, wave % MB, lane, s.cc / kScale, s.cb);
-                store_columns(poly, bj, wave % MB, lane, b[i]);
             }
+            if constexpr (MODE == kWhole)
+                __syncthreads();  // b A + c A A goes where A lies
+#pragma unroll
+            for (int i = 0; i < kSquareBlocks; ++i)
+                store_columns(poly, wave / MB * kSquareBlocks + i, wave % MB, lane, b[i]);
             __syncthreads();
             const bool last = MODE == kLast || (MODE == kWhole && k == s.steps);
             const int rb = wave % MB, cb0 = wave / MB * kStripBlocks;
@@ -275,12 +312,15 @@ __global__ __launch_bounds__(MB == 4 ? 512 : 256, 2) void muon_slim_kernel(const
                 return;
             }
             __syncthreads();  // every wave has read its blocks of X and of b A + c A A
-            rows.base = lds + kFirstRegion;
+            rows.base = lds + (MODE == kWhole ? kStrip : kFirstRegion);
 #pragma unroll
             for (int i = 0; i < kStripBlocks; ++i)
             {
                 store_columns(xt, rb0 + cb0 + i, rb, lane, x[i]);
-                store_mirror(rows, rb, cb0 + i, lane, x[i], scratch);
+                if constexpr (MODE == kWhole)
+                    store_mirror_halves(rows, rb, cb0 + i, lane, x[i], scratch);
+                else
+                    store_mirror(rows, rb, cb0 + i, lane, x[i], scratch);
             }
         }
         __syncthreads();
