@@ -123,21 +123,18 @@ struct XSource
     const float *x;
     int64_t K;
     Labels labels;
-    float scale;
     __device__ float operator()(int64_t n, int64_t k) const
     {
         if (labels(n) < 0)
             return 0.f;  // a row that does not count may hold NaN: nothing of it enters a sum
-        const float v = x[n * K + k] * scale;
-        return v;
+        return x[n * K + k];
     }
 };
 struct WSource
 {
     const float *w;
     int64_t ld, col0;
-    float scale;
-    __device__ float operator()(int64_t r, int64_t c) const { return w[r * ld + col0 + c] * scale; }
+    __device__ float operator()(int64_t r, int64_t c) const { return w[r * ld + col0 + c]; }
 };
 
 __global__ __launch_bounds__(kBlock) void ce_prepare_kernel(const PrepArgs a)
@@ -146,28 +143,32 @@ __global__ __launch_bounds__(kBlock) void ce_prepare_kernel(const PrepArgs a)
     __shared__ float scratch[4];
     int bid = (int)blockIdx.x;
     const int nx = a.x_tiles_r * a.x_tiles_c, nw = a.w_tiles_r * a.w_tiles_c;
-    if (a.mags && bid == 0)
-    {
-        const float sx = scale_from(a.mags, a.mags_x, scratch), sw = scale_from(a.mags + a.mags_x, a.mags_w, scratch);
-        if (threadIdx.x == 0)
-            a.saved[kScaleX] = sx, a.saved[kScaleW] = sw;
-    }
     if (bid < nx)
     {
-        const float s = a.mags ? scale_from(a.mags, a.mags_x, scratch) : a.saved[kScaleX];
-        split_tile(XSource{a.x, a.K, a.labels, s}, a.N, a.K, (int64_t)(bid / a.x_tiles_c) * 64, (int64_t)(bid % a.x_tiles_c) * 64, a.xr,
+        const auto factor = [&] {
+            const float s = a.mags ? scale_from(a.mags, a.mags_x, scratch) : a.saved[kScaleX];
+            if (a.mags && blockIdx.x == 0 && threadIdx.x == 0)
+                a.saved[kScaleX] = s;
+            return s;
+        };
+        split_tile(XSource{a.x, a.K, a.labels}, factor, a.N, a.K, (int64_t)(bid / a.x_tiles_c) * 64, (int64_t)(bid % a.x_tiles_c) * 64, a.xr,
                    a.xt, tile);
         return;
     }
     bid -= nx;
     if (bid < nw)
     {
-        const float s = a.mags ? scale_from(a.mags + a.mags_x, a.mags_w, scratch) : a.saved[kScaleW];
+        const auto factor = [&] {
+            const float s = a.mags ? scale_from(a.mags + a.mags_x, a.mags_w, scratch) : a.saved[kScaleW];
+            if (a.mags && bid == 0 && threadIdx.x == 0)
+                a.saved[kScaleW] = s;
+            return s;
+        };
         const int64_t r0 = (int64_t)(bid / a.w_tiles_c) * 64, c0 = (int64_t)(bid % a.w_tiles_c) * 64;
         if (a.w_out_in)
-            split_tile(WSource{a.w + a.v0 * a.K, a.K, 0, s}, a.vn, a.K, r0, c0, a.wr, a.wt, tile);
+            split_tile(WSource{a.w + a.v0 * a.K, a.K, 0}, factor, a.vn, a.K, r0, c0, a.wr, a.wt, tile);
         else
-            split_tile(WSource{a.w, a.V, a.v0, s}, a.K, a.vn, r0, c0, a.wt, a.wr, tile);
+            split_tile(WSource{a.w, a.V, a.v0}, factor, a.K, a.vn, r0, c0, a.wt, a.wr, tile);
         return;
     }
     bid -= nw;
@@ -276,7 +277,7 @@ __global__ __launch_bounds__(kBlock) void ce_join_kernel(const float *__restrict
     const int r = threadIdx.x % kJoinRows, g = threadIdx.x / kJoinRows;
     const int64_t n = (int64_t)blockIdx.x * kJoinRows + r;
     float m = -INFINITY, s = 0.f;
-#pragma unroll 4
+#pragma unroll 8
     for (int64_t t = g; t < tiles; t += 16)
         merge(m, s, part_m[t * n_pad + n], part_s[t * n_pad + n]);
     sm[g][r] = m, ss[g][r] = s;

@@ -40,12 +40,11 @@ struct Update
     }
 };
 
-struct ScaledUpdate
+struct UpdateAt
 {
     Update u;
     int64_t cols;
-    double factor;
-    __device__ float operator()(int64_t r, int64_t c) const { return (float)((double)u(r * cols + c) * factor); }
+    __device__ float operator()(int64_t r, int64_t c) const { return u(r * cols + c); }
 };
 
 // the accumulator block as rows of the other side: through the wave's scratch

@@ -73,9 +73,9 @@ __global__ __launch_bounds__(kBlock) void muon_prepare_kernel(const Matrices a, 
     __shared__ float tile[64][65];
     __shared__ double part[4];
     const int z = blockIdx.z;
-    const double norm = sqrt(sum_of_parts<4>(sums + (int64_t)z * parts, parts, part));
     r.base += z * batch_bytes, t.base += z * batch_bytes;
-    split_tile(ScaledUpdate{{a.g[z], a.buf[z], a.momentum, a.nesterov}, a.cols, (double)kScale / (norm + eps)}, a.rows, a.cols, (int64_t)blockIdx.y * 64, (int64_t)blockIdx.x * 64, r, t, tile);
+    const auto factor = [&] { return (double)kScale / (sqrt(sum_of_parts<4>(sums + (int64_t)z * parts, parts, part)) + eps); };
+    split_tile(UpdateAt{{a.g[z], a.buf[z], a.momentum, a.nesterov}, a.cols}, factor, a.rows, a.cols, (int64_t)blockIdx.y * 64, (int64_t)blockIdx.x * 64, r, t, tile);
 }
 
 // A = X X^T (prev null), or b A + c A A: symmetric, computed for tile row <= tile column

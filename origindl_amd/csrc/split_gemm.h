@@ -644,10 +644,11 @@ inline int launch_whole_gemm(const GemmArgs &args, int64_t rows_pad, int64_t col
 }
 
 // Values [rows, cols] into panels: `r` has the matrix's rows as rows, `t` its columns (either may have a null base). Src gives
-// the value at (row, col) in bounds, already scaled; a workgroup of 256 threads takes 64 x 64 values through LDS. Rows and
+// the value at (row, col) in bounds, and factor() what all are multiplied by (every thread calls it once, when its values are
+// under way: it may take its own time); a workgroup of 256 threads takes 64 x 64 values through LDS. Rows and
 // columns up to the padded extents are written as zeros.
-template <class Src>
-__device__ inline void split_tile(const Src &src, int64_t rows, int64_t cols, int64_t r0, int64_t c0, const Panel &r, const Panel &t,
+template <class Src, class Factor>
+__device__ inline void split_tile(const Src &src, const Factor &factor, int64_t rows, int64_t cols, int64_t r0, int64_t c0, const Panel &r, const Panel &t,
                                   float (*tile)[65])
 {
     const int tid = threadIdx.x;
@@ -660,9 +661,10 @@ __device__ inline void split_tile(const Src &src, int64_t rows, int64_t cols, in
             const int64_t row = r0 + (tid >> 6) + 4 * i, col = c0 + c;
             v[i] = row < rows && col < cols ? src(row, col) : 0.f;
         }
+        const auto by = factor();
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            tile[(tid >> 6) + 4 * i][c] = v[i];
+            tile[(tid >> 6) + 4 * i][c] = (float)(v[i] * by);
     }
     __syncthreads();
     const int lane = tid & 63;
