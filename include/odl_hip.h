@@ -351,7 +351,8 @@ int odl_hip_softmax_ce_loss_grad_device(const float *x, const void *t, int idx_i
  * Unlike odl_hip_softmax_ce_loss the probability is not offset by 1e-8 before the logarithm: the loss is the exact negative
  * log-likelihood and the gradient its derivative. Products are float32 in accuracy (each operand as two float16 numbers,
  * three products, float32 sums): an operand's elements are kept to 2^-22 of themselves, or to 2^-40 of the largest one where
- * that is more (the gradients' operand softmax - one-hot: to 2^-40). Neither call synchronises or allocates; both can be captured.
+ * that is more (the gradients' operand softmax - one-hot: to 2^-40). Up to 256 rows over 6 million weights or more the operands
+ * are three bfloat16 numbers instead, exact, and six products. Neither call synchronises or allocates; both can be captured.
  * forward: device_saved8[0] the loss, [1] (an int) nonzero if a label that is not ignore_index lies outside [0, V) — such a
  * row is left out like an ignored one, the caller decides when to look —, [2] the number of counted rows, the rest and
  * row_stats[N, 2] (base-2 logarithm of the row's largest exp(z), sum of exp(z) over that) are for the backward pass.
@@ -660,7 +661,8 @@ int odl_hip_sgd_step_multi_decay(int count, const float *const *p, float *const 
  * newton_schulz: out = X after `steps` of X <- a X + (b A + c A A) X, A = X X^T, from X0 = g / (||g||_F + eps), on the side of
  * the shorter dimension, for `batch` dense matrices g[batch, rows, cols]. (a, b, c) = (3.4445, -4.775, 2.0315) brings the
  * singular values to about [0.7, 1.2] in five steps. Coefficients under which they, or b A + c A A, could pass 7.5 on the way
- * are refused. Elements of X are kept to 2^-22 of themselves or 2^-38. A zero matrix gives zeros; a matrix with an infinity or a NaN gives NaN. out may be g.
+ * are refused. Elements of X are kept to 2^-22 of themselves or 2^-38. A zero matrix gives zeros; a matrix with an infinity or
+ * a NaN gives NaN. out may be g.
  * muon_step_multi: one optimiser step over a list of matrices [host_rows[i], host_cols[i]]; equal shapes go through the same
  * launches, up to 32 together:
  *   buf = momentum * buf + g;  u = nesterov ? g + momentum * buf : buf;  O = newton_schulz(u)

@@ -20,8 +20,9 @@
 //
 // The product. A workgroup holds a BM x BN tile; four stages of one contraction block each travel into LDS by direct loads
 // (no registers), queued four stages ahead; fragments of the next block are read while the present block multiplies. A
-// stage's three products use 4 fragments a pair of blocks where a plain float16 product reads 2 for one, so LDS needs only
-// half of its bandwidth.
+// stage's three products use 4 fragments a pair of blocks where a plain float16 product reads 2 for one: two thirds of the LDS
+// reads per matrix instruction. What bounds it is the chip's power: 425 to 456 TFLOP/s of float32 products, 1.3 PFLOP/s of
+// matrix instructions, whichever large tile is taken (the library's float16 product: 1.1 to 1.2; its float32 product: 0.15).
 #pragma once
 #include <algorithm>
 #include <type_traits>
@@ -491,8 +492,10 @@ struct Cut
 // TFLOP/s at which many of them run into the chip's power limit (long symmetric products lower: their tiles share less),
 // and microseconds a round of tiles spends outside its loop. Large tiles read their operands less often and leave compute
 // units idle in a short last round. Runs of the contraction (may_split) cost a pass over the partial results: out_bytes
-// written per run, read once. exact: only tiles with accumulators apart for the cross terms. For example 4096 x 4096 x 4096: 323 us with 256 x 256, 325 with 256 x 128, 333 with 128 x 128, 404
-// with 64 x 64; 1024 x 1024 x 1024: 52, 29, 19 and 8.6 us.
+// written per run, read once. exact: only tiles with accumulators apart for the cross terms. For example 4096 x 4096 x 4096:
+// 323 us with 256 x 256, 325 with 256 x 128, 333 with 128 x 128, 404 with 64 x 64; 1024 x 1024 x 1024: 52, 29, 19 and 8.6 us.
+// A short last round of tiles is left as it is: computed as smaller tiles in runs (4096 x 4096 symmetric products, 16 of 528
+// tiles) it saved nothing, because a chip at its power limit makes up for idle compute units with its clock.
 inline Cut pick_cut(int64_t rows_pad, int64_t cols_pad, bool symmetric, int64_t batch, int nkb, bool may_split = false, double out_bytes = 0,
                     bool exact = false)
 {
