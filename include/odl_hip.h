@@ -667,7 +667,7 @@ int odl_hip_sgd_step_multi_decay(int count, const float *const *p, float *const 
  * launches, up to 32 together:
  *   buf = momentum * buf + g;  u = nesterov ? g + momentum * buf : buf;  O = newton_schulz(u)
  *   p_out = p * (1 - lr * weight_decay) - lr * sqrt(max(1, rows / cols)) * O
- * buf is updated in place, p_out may be p; the same buffer must not stand for two entries. Empty matrices are skipped.
+ * buf is updated in place, p_out may be p; a buf or a p_out that stands for two entries is refused. Empty matrices are skipped.
  * Sides up to 2^20, 1 to 100 steps. Neither call synchronises or allocates device memory; both can be captured. */
 int odl_hip_newton_schulz(const float *g, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c,
                           float eps, float *out, void *workspace, size_t workspace_bytes, void *stream);

@@ -361,7 +361,12 @@ extern "C" int odl_hip_muon_step_multi(int count, const float *const *p, const f
     {
         if (int rc = check_common(who, host_rows[i], host_cols[i], i == 0 ? steps : 1, i == 0 ? a : 1.f, i == 0 ? b : 0.f, i == 0 ? c : 0.f, eps))
             return rc;
-        ODL_REQUIRE(host_rows[i] * host_cols[i] == 0 || (p[i] && g[i] && buf[i] && p_out[i]), "%s: null pointer for entry %d", who, i);
+        if (host_rows[i] * host_cols[i] == 0)
+            continue;
+        ODL_REQUIRE(p[i] && g[i] && buf[i] && p_out[i], "%s: null pointer for entry %d", who, i);
+        for (int j = 0; j < i; ++j)
+            ODL_REQUIRE(host_rows[j] * host_cols[j] == 0 || (buf[j] != buf[i] && p_out[j] != p_out[i]),
+                        "%s: entries %d and %d write the same momentum or parameter", who, j, i);
     }
     const size_t need = odl_hip_muon_step_multi_workspace_bytes(count, host_rows, host_cols);
     ODL_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "%s: workspace of %zu bytes needed, got %zu", who, need,

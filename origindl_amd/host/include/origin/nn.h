@@ -278,7 +278,7 @@ public:
 // a parameter of two or more dimensions seen as [dim 0, the rest] with both larger than 1: a Linear's weight, a Conv2d's
 // filters, not a bias [1, out]. Per matrix: buf = momentum*buf + g; u = nesterov ? g + momentum*buf : buf;
 //   p = p*(1 - lr*weight_decay) - lr*sqrt(max(1, rows/cols)) * newton_schulz(u)
-// Matrices of equal shape go through the same launches. Settings are checked when the first step runs.
+// Matrices of equal shape go through the same launches; a parameter registered twice is stepped once. Settings are checked when the first step runs.
 struct MuonOptions
 {
     float momentum = 0.95f;

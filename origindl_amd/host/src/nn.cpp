@@ -1,6 +1,7 @@
 // Host glue above the operators: modules, layers, optimizers, device API (see origin/nn.h).
 #include "origin/nn.h"
 
+#include <algorithm>
 #include <typeinfo>
 
 #include <cmath>
@@ -683,7 +684,11 @@ void Muon::step_all(std::vector<Parameter *> &params)
     const bool capturing = cuda::is_capturing();
     std::vector<Parameter *> matrices, rest;
     for (auto *p : params)
-        (is_matrix(*p) ? matrices : rest).push_back(p);
+    {
+        auto &list = is_matrix(*p) ? matrices : rest;
+        if (std::find(list.begin(), list.end(), p) == list.end())  // registered twice (tied weights): stepped once
+            list.push_back(p);
+    }
     std::vector<OriginMat::MuonItem> items;
     std::vector<Tensor> grads;  // keeps the gradients alive until the launches are queued
     for (auto *p : matrices)
@@ -892,7 +897,7 @@ std::unordered_map<std::string, std::any> Muon::state_dict() const
     StateDict buffers;
     for (const auto &kv : momentum_buffers_)
         if (const std::string n = name_of(named, kv.first); !n.empty())
-            buffers["momentum_" + n] = kv.second;
+            buffers["momentum_" + n] = kv.second.clone();  // steps write the buffer in place: the state is that of now
     state["momentum_buffers"] = buffers;
     return state;
 }
@@ -911,6 +916,8 @@ void Muon::load_state_dict(const std::unordered_map<std::string, std::any> &sd)
     rest_.load_state_dict(rest);
     auto named = target_->named_parameters("");
     read_buffers(sd, "momentum_buffers", "momentum_", named, momentum_buffers_);
+    for (auto &kv : momentum_buffers_)
+        kv.second = kv.second.clone();
 }
 
 // The reference compares a ten-character prefix with the nine-character "momentum_" and so never restores a

@@ -1684,5 +1684,46 @@ int DRV(muon_train)(const float *x, const int64_t *t, int64_t N, int64_t D, int6
             origin::cuda::set_stream(nullptr), origin::cuda::destroy_stream(stream);
     });
 }
+
+// A module that registers its parameter p [rows, cols] `names` times, under Muon, with the gradient g in each of `steps` steps.
+// After the first step the optimizer's state is taken, and at the end its momentum is written to `kept`; a second optimizer
+// that was given the same state has taken its own step on another parameter by then.
+int DRV(muon_shared)(const float *p, const float *g, int64_t rows, int64_t cols, int names, int steps, float lr, float *o, float *kept)
+{
+    return guarded([&] {
+        struct Holder : Module
+        {
+            Parameter p;
+            Holder(const Tensor &t, int names) : p(t)
+            {
+                for (int i = 0; i < names; ++i)
+                    register_parameter("p" + std::to_string(i), p);
+            }
+            Tensor forward(const Tensor &x) override { return x; }
+        };
+        const Shape shape{(size_t)rows, (size_t)cols};
+        Holder model(f32(p, shape, true), names), other(f32(p, shape, true), 1);
+        auto G = f32(g, shape);
+        Muon opt(model, lr), second(other, lr);
+        const auto step = [&](Holder &m, Muon &by) {
+            by.zero_grad();
+            F::sum(m.p * G).backward();
+            by.step();
+        };
+        std::unordered_map<std::string, std::any> state;
+        for (int s = 0; s < steps; ++s)
+        {
+            step(model, opt);
+            if (s == 0)
+            {
+                state = opt.state_dict();
+                if (names == 1)
+                    second.load_state_dict(state), step(other, second);
+            }
+        }
+        out(model.p, o);
+        out(std::any_cast<Module::StateDict>(state.at("momentum_buffers")).begin()->second, kept);
+    });
+}
 #endif
 }  // extern "C"

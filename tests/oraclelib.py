@@ -125,6 +125,7 @@ _DEVICE_ONLY_SIGS = {
     "odl_host_linear_softmax_ce": "ppippillllfpppp>i",
     "odl_host_newton_schulz": "plllip>i",
     "odl_host_muon_train": "ppllll" "iifffpp>i",
+    "odl_host_muon_shared": "ppllii" "fpp>i",
 }
 
 

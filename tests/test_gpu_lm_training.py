@@ -556,3 +556,23 @@ def test_host_training_steps_with_muon(capi, h):
             assert float((got - w).norm()) <= scale * (schulz_bar(5) + 1e-5 * 3.4445 ** 5) + 2.0 ** -22 * float(p.norm())
         else:  # Adam's first step is adam_lr times the gradient's sign, smoothed by eps against the gradient's size
             assert bool(((got - w).abs() <= 0.02 * adam_lr).float().mean() > 0.97) and bool(((got - p.cuda().double()).abs() <= 1.01 * adam_lr).all())
+
+
+def test_host_muon_steps_a_shared_parameter_once_and_keeps_its_state(capi, h):
+    """A parameter registered under two names gives the bits of the same one registered once; the momentum in a state taken
+    after the first step is that step's, the gradient itself, whatever either optimizer has done since."""
+    rows, cols = 40, 56
+    g = torch.Generator().manual_seed(77)
+    p, q = torch.randn(rows, cols, generator=g), torch.randn(rows, cols, generator=g)
+    results = []
+    for names in (1, 2):
+        o, kept = np.empty((rows, cols), np.float32), np.empty((rows, cols), np.float32)
+        assert h.odl_host_muon_shared(p.numpy(), q.numpy(), rows, cols, names, 3, 0.05, o, kept) == 0
+        assert np.array_equal(kept, q.numpy())
+        results.append(o)
+    assert np.array_equal(results[0], results[1])
+    want, buf = p, torch.zeros_like(p)
+    for _ in range(3):
+        want, buf, _ = muon64(want, q, buf, 0.05, 0.95, True, 0.0)
+    off = float((torch.from_numpy(results[0]).double() - want).norm())
+    assert off <= 3 * (0.05 * 1.21 * rows ** 0.5 * schulz_bar(5) + 2.0 ** -22 * float(p.norm()))

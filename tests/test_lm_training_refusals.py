@@ -91,6 +91,8 @@ def test_muon_step_refuses_bad_arguments(l):
     assert muon(l, [(4, 8)], coef=(10.0, 0.0, 0.0)) == BAD and "coefficients" in l.last_error()
     assert muon(l, [(4, 8)], ws=None) == BAD and "workspace" in l.last_error()
     assert muon(l, [(4, 8)], nb=64) == BAD and "workspace" in l.last_error()
+    # one momentum for two matrices (an empty one between them writes nothing)
+    assert muon(l, [(4, 8), (0, 8), (8, 4)]) == BAD and "entries 0 and 2" in l.last_error()
 
 
 def test_muon_workspace_is_that_of_the_largest_group(l):
