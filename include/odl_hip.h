@@ -342,9 +342,10 @@ int odl_hip_softmax_ce_loss_grad_device(const float *x, const void *t, int idx_i
 
 /* A Linear layer and the cross entropy of its outputs as one operator (Linear::forward, src/nn/layers/linear.cpp:80-106,
  * then SoftmaxCrossEntropy, src/operators/loss/softmax_cross_entropy.cpp:17-111) for large vocabularies: the [N, V] logits
- * z = x[N,K] . w + b are never stored, neither in the forward nor in the backward pass, which goes over the vocabulary in
- * pieces. w is [K, V] as nn::Linear keeps it, or [V, K] with w_out_in != 0 (LinearOp's layout, src/operators/custom/linear.cpp,
- * and an embedding's); b[V] may be NULL, and may hold -inf for entries that must not be predicted.
+ * z = x[N,K] . w + b are not stored, neither in the forward nor in the backward pass, which goes over the vocabulary in
+ * pieces (only where they are small beside the weights, see row_stats). w is [K, V] as nn::Linear keeps it, or [V, K] with
+ * w_out_in != 0 (LinearOp's layout, src/operators/custom/linear.cpp, and an embedding's); b[V] may be NULL, and may hold -inf
+ * for entries that must not be predicted.
  *   loss = 1/C * sum over the C counted rows of (log sum_v exp(z[n][v]) - z[n][t[n]])
  * Rows whose label is ignore_index are not counted (pass a value no label has, e.g. -100, to count all): they add nothing to
  * the loss or to a gradient, whatever x holds there, NaN included. With no counted row the loss and all gradients are 0.
@@ -355,7 +356,9 @@ int odl_hip_softmax_ce_loss_grad_device(const float *x, const void *t, int idx_i
  * are three bfloat16 numbers instead, exact, and six products. Neither call synchronises or allocates; both can be captured.
  * forward: device_saved8[0] the loss, [1] (an int) nonzero if a label that is not ignore_index lies outside [0, V) — such a
  * row is left out like an ignored one, the caller decides when to look —, [2] the number of counted rows, the rest and
- * row_stats[N, 2] (base-2 logarithm of the row's largest exp(z), sum of exp(z) over that) are for the backward pass.
+ * row_stats are for the backward pass: [N, 2] (base-2 logarithm of the row's largest exp(z), sum of exp(z) over that), and
+ * behind them, with up to 256 rows whose logits are at most a quarter of the weights' size, the logits:
+ * odl_hip_linear_softmax_ce_row_stats_floats(N, K, V) floats in all.
  * backward: gx[N,K], gw (w's layout), gb[V], each may be NULL; the upstream gradient is read from device_gy[0] (NULL: 1).
  * x, w, b, t, saved and row_stats are the forward call's, unchanged; outputs must not overlap inputs.
  * N = 0 is an empty batch. N and K up to 2^20, V up to 2^30; the workspace's alignment is 16 bytes. */
@@ -363,6 +366,7 @@ int odl_hip_linear_softmax_ce_forward(const float *x, const float *w, int w_out_
                                       int64_t ignore_index, int64_t N, int64_t K, int64_t V, float *device_saved8,
                                       float *row_stats, void *workspace, size_t workspace_bytes, void *stream);
 size_t odl_hip_linear_softmax_ce_forward_workspace_bytes(int64_t N, int64_t K, int64_t V);
+size_t odl_hip_linear_softmax_ce_row_stats_floats(int64_t N, int64_t K, int64_t V);
 int odl_hip_linear_softmax_ce_backward(const float *device_gy, const float *x, const float *w, int w_out_in, const float *b,
                                        const void *t, int idx_is_i64, int64_t ignore_index, int64_t N, int64_t K, int64_t V,
                                        const float *device_saved8, const float *row_stats, float *gx, float *gw, float *gb,

@@ -527,7 +527,7 @@ def linear_softmax_cross_entropy(x, w, b, t, ignore_index=-100, w_out_in=False):
     linear_softmax_cross_entropy_bad_label). w: [K, V], or [V, K] with w_out_in. Does not synchronise."""
     N, K, V, is64 = _ce_args("linear_softmax_cross_entropy", x, w, b, t, w_out_in)
     with _on(x.device):
-        saved, rows = x.new_empty(8), x.new_empty((N, 2))
+        saved, rows = x.new_empty(8), x.new_empty(lib().query("odl_hip_linear_softmax_ce_row_stats_floats", N, K, V))
         ws, nb = _ws_like(x, lib().query("odl_hip_linear_softmax_ce_forward_workspace_bytes", N, K, V))
         lib().call("odl_hip_linear_softmax_ce_forward", _p(x), _p(w), int(w_out_in), _p(b), _p(t), is64, int(ignore_index), N, K, V,
                    _p(saved), _p(rows), _p(ws), nb, _stream())
@@ -546,7 +546,8 @@ def linear_softmax_cross_entropy_backward(gy, x, w, b, t, saved, ignore_index=-1
     if gy is not None and (_chk(gy, "gy").numel() != 1 or gy.device != x.device):
         raise OdlInvalidArgument("linear_softmax_cross_entropy_backward: gy must be one element on x's device")
     words, rows = _chk(saved[0], "saved"), _chk(saved[1], "saved")
-    if words.numel() != 8 or tuple(rows.shape) != (N, 2) or words.device != x.device or rows.device != x.device:
+    kept = lib().query("odl_hip_linear_softmax_ce_row_stats_floats", N, K, V)
+    if words.numel() != 8 or rows.numel() != kept or words.device != x.device or rows.device != x.device:
         raise OdlInvalidArgument("linear_softmax_cross_entropy_backward: saved is not from a forward call with %d rows" % N)
     with _on(x.device):
         gx = x.new_empty((N, K)) if need_gx else None

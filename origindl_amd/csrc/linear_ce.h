@@ -102,6 +102,7 @@ inline bool few_rows(int64_t N, int64_t K, int64_t V)
 {
     return N <= 256 && K * V >= 6000000;
 }
+size_t few_kept_floats(int64_t N, int64_t K, int64_t V);  // of logits that stay behind the row statistics
 size_t few_forward_bytes(int64_t N, int64_t K, int64_t V);
 size_t few_backward_bytes(int64_t N, int64_t K, int64_t V);
 int few_forward(const Problem &p, float *saved, float *row_stats, char *workspace, hipStream_t st);

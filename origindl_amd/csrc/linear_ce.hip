@@ -623,6 +623,13 @@ extern "C" size_t odl_hip_linear_softmax_ce_forward_workspace_bytes(int64_t N, i
     return forward_space(nullptr, make_plan(N, K, V, false), N, K, V).bytes;
 }
 
+extern "C" size_t odl_hip_linear_softmax_ce_row_stats_floats(int64_t N, int64_t K, int64_t V)
+{
+    if (N <= 0 || K <= 0 || V <= 0 || N > kMostRows || K > kMostRows || V > kMostVocabulary)
+        return 0;
+    return (size_t)(2 * N) + (few_rows(N, K, V) ? few_kept_floats(N, K, V) : 0);
+}
+
 extern "C" size_t odl_hip_linear_softmax_ce_backward_workspace_bytes(int64_t N, int64_t K, int64_t V)
 {
     if (N <= 0 || K <= 0 || V <= 0 || N > kMostRows || K > kMostRows || V > kMostVocabulary)

@@ -3,8 +3,9 @@
 // What bounds it: the bytes of w. So nothing is laid out first: w streams once from where it lies through the registers into
 // the matrix instructions, per pass:
 //   forward    one pass: logits of 128 (64) entries a workgroup, their maximum and sum of powers in its epilogue
-//   backward   one pass for the logits again, whose epilogue writes d = softmax - one-hot (the weights' size times 3N / K) and
-//              gb; one pass for gx = d.w, in runs of the vocabulary; gw = d^T.x writes its size once.
+//   backward   the logits, which the forward pass has kept if they are small beside the weights (else one pass for them again):
+//              the same epilogue in both cases writes d = softmax - one-hot (the weights' size times 3N / K) and gb; one pass for
+//              gx = d.w, in runs of the vocabulary; gw = d^T.x writes its size once.
 //
 // Mathematics. A float32 number is the sum of three bfloat16 numbers, its first, second and third eight bits, cut off without
 // rounding: exact. Of the nine products of two such sums the six of at least 2^-16 of the whole are formed by bfloat16 matrix
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(kBlock) void ce_rows_prepare_kernel(const float *__
     const int lane = threadIdx.x & 63;
     const int64_t unit = (int64_t)blockIdx.x * (kBlock / 64) + (threadIdx.x >> 6);
     float v[8];
-    if (unit < groups * blocks_n)
+    if (by_n && unit < groups * blocks_n)
     {
         const int64_t g = unit / blocks_n, n = (unit - g * blocks_n) * 32 + (lane & 31), k = g * 16 + (lane >> 5) * 8;
         const bool counts = labels(n) >= 0;
@@ -284,12 +285,22 @@ __device__ inline int place_of(int m, int lane, int e)
     return OUT_ROWS ? 32 * m + r : VB * r + m;
 }
 
+// Where a workgroup of waves m keeps its sums between the passes: [tile][workgroup of rows][block of rows][block of outputs], each
+// as a wave holds it. (The address need not be a multiple of 16.)
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+template <int VB, int NB, class F>
+__device__ inline F *kept_at(F *kept, int64_t tile, int nb0, int blocks_n, int nb, int m, int lane)
+{
+    return kept + ((tile * (blocks_n / NB) + nb0 / NB) * NB + nb) * (VB * 1024) + m * 1024 + lane * 4;
+}
+
 struct RowsStatsEpilogue
 {
     const float *b;
     Labels labels;
     int64_t V;
     float *part_m, *part_s, *target;
+    float *kept;  // null, or where x.w stays for the backward pass (rows past the batch are left out)
     template <int VB, int NB, bool OUT_ROWS>
     __device__ void run(int64_t tile, int nb0, int blocks_n, int m, int lane, f32x16 *z, float *lds) const
     {
@@ -308,6 +319,13 @@ struct RowsStatsEpilogue
             {
                 const int64_t n = (nb0 + nb) * 32 + (lane & 31), label = labels(n) - tile * (32 * VB);
                 float top = -INFINITY;
+                if (kept && n < labels.N)
+                {
+                    float *at = kept_at<VB, NB>(kept, tile, nb0, blocks_n, nb, m, lane);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<f32x4u *>(at + i * 256) = f32x4{z[nb][4 * i], z[nb][4 * i + 1], z[nb][4 * i + 2], z[nb][4 * i + 3]};
+                }
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                 {
@@ -428,6 +446,29 @@ struct RowsGradEpilogue
         }
     }
 };
+
+// the pass over w for the logits, where the forward pass has kept them
+template <int VB, int NB, bool OUT_ROWS, class Epilogue>
+__global__ __launch_bounds__(64 * kWaves) void ce_kept_kernel(const float *__restrict__ kept, int blocks_n, const Epilogue epilogue)
+{
+    __shared__ float lds[32 * VB * (32 * NB + 1)];
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    const unsigned per_tile = (unsigned)(blocks_n / NB), tile = blockIdx.x / per_tile;
+    const int nb0 = (int)(blockIdx.x - tile * per_tile) * NB;
+    f32x16 sum[NB];
+    if (wave < VB)
+    {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+            {
+                const f32x4 v  = *reinterpret_cast<const f32x4u *>(kept_at<VB, NB>(kept, tile, nb0, blocks_n, nb, wave, lane) + i * 256);
+                sum[nb][4 * i] = v[0], sum[nb][4 * i + 1] = v[1], sum[nb][4 * i + 2] = v[2], sum[nb][4 * i + 3] = v[3];
+            }
+    }
+    epilogue.template run<VB, NB, OUT_ROWS>(tile, nb0, blocks_n, wave, lane, sum, lds);
+}
 
 // parts[run][feature][rows]
 struct RowsPartEpilogue
@@ -628,6 +669,25 @@ int stream(const float *w, bool out_rows, int64_t ld, int64_t outs, int64_t cont
     return ODL_OK;
 }
 
+template <class Epilogue>
+int from_kept(const float *kept, bool out_rows, int64_t outs, int blocks_n, const Epilogue &e, hipStream_t st)
+{
+    const int64_t blocks = odl::ceil_div(outs, tile_of(blocks_n)) * (blocks_n / taken_of(blocks_n));
+    ODL_REQUIRE(blocks < ((int64_t)1 << 31), "linear_softmax_ce: too many tiles");
+    const dim3 grid((unsigned)blocks), block(64 * kWaves);
+    switch (taken_of(blocks_n) * 2 + (out_rows ? 1 : 0))
+    {
+        case 2: ce_kept_kernel<4, 1, false, Epilogue><<<grid, block, 0, st>>>(kept, blocks_n, e); break;
+        case 3: ce_kept_kernel<4, 1, true, Epilogue><<<grid, block, 0, st>>>(kept, blocks_n, e); break;
+        case 4: ce_kept_kernel<4, 2, false, Epilogue><<<grid, block, 0, st>>>(kept, blocks_n, e); break;
+        case 5: ce_kept_kernel<4, 2, true, Epilogue><<<grid, block, 0, st>>>(kept, blocks_n, e); break;
+        case 8: ce_kept_kernel<2, 4, false, Epilogue><<<grid, block, 0, st>>>(kept, blocks_n, e); break;
+        default: ce_kept_kernel<2, 4, true, Epilogue><<<grid, block, 0, st>>>(kept, blocks_n, e); break;
+    }
+    ODL_LAUNCH_CHECK();
+    return ODL_OK;
+}
+
 // whole tiles of 128 features: a tile of gw reads them all
 int prepare(const Problem &p, int blocks_n, u32x4 *by_n, u32x4 *by_k, float *saved, hipStream_t st)
 {
@@ -653,13 +713,21 @@ size_t few_backward_bytes(int64_t N, int64_t K, int64_t V)
     return ::backward_space(nullptr, N, K, V).bytes;
 }
 
+// The logits stay where they are at most a quarter of the weights, which the backward pass would read again for them.
+size_t few_kept_floats(int64_t N, int64_t K, int64_t V)
+{
+    const int64_t rows = blocks_of(N) * 32, tile = tile_of(blocks_of(N));
+    return 4 * rows <= K ? (size_t)(ceil_div(V, tile) * tile * rows) : 0;
+}
+
 int few_forward(const Problem &p, float *saved, float *row_stats, char *workspace, hipStream_t st)
 {
     const int blocks_n = blocks_of(p.N);
     const FewSpace s   = ::forward_space(workspace, p.N, p.K, p.V);
     if (int rc = prepare(p, blocks_n, s.x_by_n, nullptr, saved, st))
         return rc;
-    const RowsStatsEpilogue e{p.b, p.labels, p.V, s.part_m, s.part_s, s.target};
+    float *kept = few_kept_floats(p.N, p.K, p.V) ? row_stats + 2 * p.N : nullptr;
+    const RowsStatsEpilogue e{p.b, p.labels, p.V, s.part_m, s.part_s, s.target, kept};
     if (int rc = stream(p.w, p.w_out_in != 0, p.w_out_in ? p.K : p.V, p.V, p.K, s.x_by_n, blocks_n, 1, e, st))
         return rc;
     return join(s.part_m, s.part_s, s.target, ceil_div(p.V, tile_of(blocks_n)), blocks_n * 32, p.labels, row_stats, s.join_scratch, saved, st);
@@ -670,11 +738,14 @@ int few_backward(const Problem &p, const float *gy, const float *saved, const fl
 {
     const int blocks_n = blocks_of(p.N);
     const FewSpace s   = ::backward_space(workspace, p.N, p.K, p.V);
-    if (int rc = prepare(p, blocks_n, s.x_by_n, gw ? s.x_by_k : nullptr, nullptr, st))
-        return rc;
+    const bool kept    = few_kept_floats(p.N, p.K, p.V) != 0;
+    if (gw || !kept)
+        if (int rc = prepare(p, blocks_n, kept ? nullptr : s.x_by_n, gw ? s.x_by_k : nullptr, nullptr, st))
+            return rc;
     const int64_t ld = p.w_out_in ? p.K : p.V;
     const RowsGradEpilogue e{p.b, saved, row_stats, p.labels, p.V, gx ? s.d_by_n : nullptr, gw ? s.d_by_v : nullptr, gb ? s.sums : nullptr};
-    if (int rc = stream(p.w, p.w_out_in != 0, ld, p.V, p.K, s.x_by_n, blocks_n, 1, e, st))
+    if (int rc = kept ? from_kept(row_stats + 2 * p.N, p.w_out_in != 0, p.V, blocks_n, e, st)
+                      : stream(p.w, p.w_out_in != 0, ld, p.V, p.K, s.x_by_n, blocks_n, 1, e, st))
         return rc;
     if (gb)
     {

@@ -2286,7 +2286,7 @@ std::unique_ptr<Mat> OriginMat::linear_softmax_cross_entropy(const Mat &w_, cons
     const bool known = t.storage()->int_range(&lo, &hi) && ((lo >= 0 && hi < V) || (lo == ignore_index && hi == ignore_index));
     Workspace ws(odl_hip_linear_softmax_ce_forward_workspace_bytes(N, K, V), device().index());
     auto storage = Storage::create(kLinearCeWords * sizeof(float), DeviceType::kCUDA, device().index());
-    auto stats   = std::make_unique<OriginMat>(Shape{(size_t)N, 2}, DataType::kFloat32, device());
+    auto stats   = std::make_unique<OriginMat>(Shape{odl_hip_linear_softmax_ce_row_stats_floats(N, K, V)}, DataType::kFloat32, device());
     check(odl_hip_linear_softmax_ce_forward(fp(x), fp(w), w_out_in, b ? fp(*b) : nullptr, t.storage()->data(), is64, ignore_index, N, K, V,
                                             static_cast<float *>(storage->data()), stats->data_ptr<float>(), ws.ptr(), ws.bytes, cur()));
     auto loss = std::make_unique<OriginMat>(std::move(storage), Shape{}, DataType::kFloat32);
