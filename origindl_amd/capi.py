@@ -522,7 +522,7 @@ def _ce_args(who, x, w, b, t, w_out_in):
 
 
 def linear_softmax_cross_entropy(x, w, b, t, ignore_index=-100, w_out_in=False):
-    """Mean cross entropy of softmax(x . w + b) without storing the logits -> (loss, saved): loss a 0-dim device tensor,
+    """Mean cross entropy of softmax(x . w + b) without storing large logits -> (loss, saved): loss a 0-dim device tensor,
     saved = (words, row_stats) for the backward pass; words[1] viewed as int32 is nonzero after a label out of range (see
     linear_softmax_cross_entropy_bad_label). w: [K, V], or [V, K] with w_out_in. Does not synchronise."""
     N, K, V, is64 = _ce_args("linear_softmax_cross_entropy", x, w, b, t, w_out_in)

@@ -12,8 +12,8 @@
 // instructions (v_mfma_f32_32x32x16_bf16), exact in float32, and summed there: what is left out is under 2^-23 of |a||b|. No
 // scale is needed, as bfloat16 has float32's exponents, and so no pass over w to find one. Six products take 0.38 of the float32
 // matrix instruction's time. Measured: one row over 2048 x 32000, the forward pass streams 262 MB in 47 to 52 us (5.0 to 5.5
-// TB/s; a copy of 4 GiB reaches 4.8); over 2048 x 100000, forward and backward, 8 rows 886 us, 64 rows 1092, 128 rows 1651,
-// 256 rows 2882: past 64 rows the splitting and the products take longer than the bytes.
+// TB/s; a copy of 4 GiB reaches 4.8); over 2048 x 100000, forward and backward, 8 rows 692 us, 64 rows 875, 128 rows 1340,
+// 256 rows 2346: past 64 rows the splitting and the products take longer than the bytes.
 //
 // Both products with w are one kernel: w is [out][contraction] for the logits of a [V, K] weight and [contraction][out] for its
 // gx, and the other way round for a [K, V] weight. Eight waves share a tile of outputs, each takes an eighth of the contraction,
@@ -140,8 +140,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void ce_stream_kernel(const Stream 
 #pragma unroll
             for (int e = 0; e < 16; ++e)
                 acc[m][nb][e] = 0.f;
-    // Along rows of w the waves take steps in turn: together they read 512 consecutive bytes of a row (with an eighth of the row
-    // each, 64 bytes at a time, 2048 x 100000 took X us for 183 now). Down columns each takes rows of its own.
+    // Along rows of w the waves take steps in turn: together they read 512 consecutive bytes of a row (one row over
+    // [32000, 1024]: 40 us; with an eighth of the row each, 64 bytes at a time, 54). Down columns each takes rows of its own.
+    // (Workgroups that start at different places of their rows were slower, [100000, 2048]: 251 -> 283 us.)
     constexpr int kTurn  = OUT_ROWS ? kWaves : 1;
     const int64_t base   = (int64_t)blockIdx.y * kWaves * a.wave_groups;
     const int64_t first  = base + (OUT_ROWS ? wave : wave * a.wave_groups);

@@ -120,8 +120,8 @@ Tensor softmax_cross_entropy(const Tensor &x, const Tensor &target);
 // throws std::invalid_argument for one, as the reference's gather does; a recorded step cannot). `loss` is the tensor
 // softmax_cross_entropy returned while the step was recorded. Reads two words back from the device.
 bool softmax_cross_entropy_bad_label(const Tensor &loss);
-// softmax_cross_entropy(linear(x, weight, bias), target) for large vocabularies: the logits of x[N, K] are never stored,
-// neither here nor in backward. weight is [K, V] as nn::Linear keeps it, or [V, K] (LinearOp's layout, an embedding's) with
+// softmax_cross_entropy(linear(x, weight, bias), target) for large vocabularies: the logits of x[N, K] are not stored
+// (unless they are small beside the weights), neither here nor in backward. weight is [K, V] as nn::Linear keeps it, or [V, K] (LinearOp's layout, an embedding's) with
 // weight_out_in; bias (may be null) has V values. Rows whose target is ignore_index do not count: not in the mean, not in a
 // gradient, whatever x holds there; without a counted row the loss is 0. The probability is not offset before the logarithm.
 // A target outside [0, V) that is not ignore_index throws; while a step is being recorded it cannot, and

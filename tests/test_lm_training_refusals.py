@@ -53,6 +53,15 @@ def test_output_layer_workspaces_are_bounded(l):
         assert q(8192, 2048, 512000) - q(8192, 2048, 128000) <= per_entry * 384000 + (64 << 20)
 
 
+def test_row_statistics_hold_logits_only_where_they_are_small(l):
+    q = lambda N, K, V: l.query("odl_hip_linear_softmax_ce_row_stats_floats", N, K, V)
+    assert q(0, 8, 8) == q(4, 0, 8) == q(4, 8, -1) == 0
+    assert q(4, 8, 16) == 8 and q(4096, 1024, 32000) == 8192  # small weights; many rows
+    assert q(256, 515, 12007) == 512                          # few rows whose logits are half the weights
+    for N, K, V in ((1, 2048, 32000), (7, 129, 50003), (64, 2000, 4001), (128, 1031, 60021), (256, 1024, 100000)):
+        assert 2 * N + N * V <= q(N, K, V) <= 2 * N + (K * V) // 4 + 128 * 256, (N, K, V)
+
+
 def schulz(l, batch=1, rows=4, cols=8, steps=5, coef=COEF, eps=1e-7, g=SOME, out=SOME, ws=SOME, nb=None):
     nb = l.query("odl_hip_newton_schulz_workspace_bytes", batch, rows, cols) if nb is None else nb
     return l.cdll.odl_hip_newton_schulz(g, batch, rows, cols, steps, *coef, eps, out, ws, nb, None)
