@@ -96,8 +96,8 @@ struct Problem
 // Few rows over large weights: the bytes of the weights are what a pass costs, and they are read as they lie, no operand laid out
 // first. Measured with one row over 2048 x 32000: forward 61 us against 306; over 2048 x 100000, forward and backward, 64 rows
 // 875 us against 1364, 128 rows 1340 against 2503. A tile of the streams holds 32, 64 or 128 rows, and a part of one costs the
-// whole. With 64 rows over 256 x 1000 the operands laid out win, 68 us against 98: their
-// launches fill the chip where the streams' tiles of 128 entries do not. The estimates of both cross at about 6 million weights.
+// whole. With 64 rows over 256 x 1000 the operands laid out win, 68 us against 98: their launches fill the chip where the
+// streams' tiles of 128 entries do not. The estimates of both cross at about 6 million weights.
 inline bool few_rows(int64_t N, int64_t K, int64_t V)
 {
     return N <= 256 && K * V >= 6000000;
