@@ -455,34 +455,48 @@ struct OutEpilogue
     }
 };
 
-// gx: the runs of the contraction added up in order
-__global__ __launch_bounds__(kBlock) void ce_add_parts_kernel(const float *__restrict__ parts, int count, int64_t n, float *__restrict__ out)
+// What is added up after the products of a piece, in one launch. First gb[v]: the partial sums of the tiles' column waves in
+// order, 64 entries a workgroup.
+struct BiasGrad
 {
-    for (int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x; i < n; i += (int64_t)gridDim.x * kBlock)
+    const float *sums;
+    int parts;
+    int64_t v_pad, vn;
+    float *gb;
+    const float *saved, *gy;
+    __device__ void operator()(unsigned block) const
+    {
+        __shared__ float part[4][64];
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int64_t v = (int64_t)block * 64 + lane;
+        float s = 0.f;
+        for (int p = wave; p < parts; p += 4)
+            s += sums[(int64_t)p * v_pad + v];
+        part[wave][lane] = s;
+        __syncthreads();
+        if (wave == 0 && v < vn)
+        {
+            s = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+            gb[v] = s / kDScale * ((gy ? *gy : 1.f) / fmaxf(saved[kCounted], 1.f));
+        }
+    }
+};
+
+// Then, after the last piece, gx: the runs of the contraction in order, by the workgroups from bias_blocks on.
+__global__ __launch_bounds__(kBlock) void ce_sums_kernel(const BiasGrad bias, unsigned bias_blocks, const float *__restrict__ parts, int count, int64_t n,
+                                                         float *__restrict__ out)
+{
+    if (blockIdx.x < bias_blocks)
+    {
+        bias(blockIdx.x);
+        return;
+    }
+    for (int64_t i = (int64_t)(blockIdx.x - bias_blocks) * kBlock + threadIdx.x; i < n; i += (int64_t)(gridDim.x - bias_blocks) * kBlock)
     {
         float s = parts[i];
         for (int p = 1; p < count; ++p)
             s += parts[(int64_t)p * n + i];
         out[i] = s;
-    }
-}
-
-// gb[v] of a piece: the partial sums of the tiles' column waves in order
-__global__ __launch_bounds__(kBlock) void ce_bias_grad_kernel(const float *__restrict__ sums, int parts, int64_t v_pad, int64_t vn, const float *saved, const float *gy,
-                                                              float *__restrict__ gb)
-{
-    __shared__ float part[4][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t v = (int64_t)blockIdx.x * 64 + lane;
-    float s = 0.f;
-    for (int p = wave; p < parts; p += 4)
-        s += sums[(int64_t)p * v_pad + v];
-    part[wave][lane] = s;
-    __syncthreads();
-    if (wave == 0 && v < vn)
-    {
-        s = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
-        gb[v] = s / kDScale * ((gy ? *gy : 1.f) / fmaxf(saved[kCounted], 1.f));
     }
 }
 
@@ -766,19 +780,16 @@ extern "C" int odl_hip_linear_softmax_ce_backward(const float *device_gy, const 
             if (int rc = launch_gemm(product(s.dt, s.wt, vn), p.n_pad, p.k_pad, gx_cut, o, st))
                 return rc;
         }
-        if (gb)
+        const int64_t n            = N * K;
+        const unsigned bias_blocks = gb ? (unsigned)(v_pad / 64) : 0u;
+        const unsigned gx_blocks   = gx && p.gx.splits > 1 && i + 1 == p.pieces ? (unsigned)std::min<int64_t>(2048, odl::ceil_div(n, kBlock)) : 0u;
+        if (bias_blocks + gx_blocks)
         {
             const int waves_n = cut.bn == 256 ? 4 : 2;
-            ce_bias_grad_kernel<<<dim3((unsigned)(v_pad / 64)), dim3(kBlock), 0, st>>>(s.sums, (int)(p.n_pad / cut.bn) * waves_n, v_pad, vn, saved8, device_gy,
-                                                                                       gb + v0);
+            const BiasGrad bias{s.sums, (int)(p.n_pad / cut.bn) * waves_n, v_pad, vn, gb ? gb + v0 : nullptr, saved8, device_gy};
+            ce_sums_kernel<<<dim3(bias_blocks + gx_blocks), dim3(kBlock), 0, st>>>(bias, bias_blocks, s.parts, p.gx.splits, n, gx);
             ODL_LAUNCH_CHECK();
         }
-    }
-    if (gx && p.gx.splits > 1)
-    {
-        const int64_t n = N * K;
-        ce_add_parts_kernel<<<dim3((unsigned)std::min<int64_t>(2048, odl::ceil_div(n, kBlock))), dim3(kBlock), 0, st>>>(s.parts, p.gx.splits, n, gx);
-        ODL_LAUNCH_CHECK();
     }
     return ODL_OK;
 }
