@@ -8,9 +8,10 @@
 //             gw = d^T.x); the sums over tokens for gb come out of the same epilogue.
 //
 // What bounds it: matrix products, 2NKV operations forward and 6NKV backward (the logits a second time: 4NKV with logits
-// kept), each as three float16 products (split_gemm.h). Exponentials: one per logit and direction. Measured, 8192 tokens x 1024
-// over 32000 entries: forward's product 2.9 ms of 3.1 (profiled), the rate at which the chip's power lets the matrix
-// instructions run; 2048 tokens, both directions: 2.97 ms, of it 0.15 to lay out operands and 0.06 for sums and joins.
+// kept), each as three float16 products (split_gemm.h). Exponentials: one per logit and direction. Measured, 16384 tokens x 1024
+// over 32000 entries: loss 2.63 to 2.74 ms, 392 to 408 TFLOP/s of all, 0.17 ms of it to find scales, lay out operands and join;
+// 4096 tokens, both directions: 2.97 to 3.06 ms, of it 0.17 to lay out and 0.05 for sums and joins. The rest are products at
+// the rate that the chip's power allows.
 //
 // In the products the vocabulary is the row side: a lane's accumulators then belong to one token, and the maximum and the
 // sum over the vocabulary are sums over a lane's own registers, one exchange between the wave's halves and one through LDS.
