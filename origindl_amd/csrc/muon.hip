@@ -215,7 +215,8 @@ Space space_for(char *base, int count, int64_t rows, int64_t cols)
     return s;
 }
 
-// how many equal matrices go through the launches together: what 2 GiB of workspace holds
+// how many equal matrices go through the launches together: what 2 GiB of workspace holds. The last group of a call may be
+// smaller, and its products cut into more runs than the full group's: either may need the larger workspace.
 int group_of(int count, int64_t rows, int64_t cols)
 {
     const int64_t each = space_for(nullptr, 1, rows, cols).batch_bytes;
@@ -256,9 +257,12 @@ int check_common(const char *who, int64_t rows, int64_t cols, int steps, float a
     return ODL_OK;
 }
 
-int run_group(const Matrices &mat, int count, int steps, float a, float b, float c, float eps, float keep, float rate, char *workspace, hipStream_t st)
+int run_group(const char *who, const Matrices &mat, int count, int steps, float a, float b, float c, float eps, float keep, float rate, void *workspace,
+              size_t workspace_bytes, hipStream_t st)
 {
-    const Space s = space_for(workspace, count, mat.rows, mat.cols);
+    const Space s = space_for(static_cast<char *>(workspace), count, mat.rows, mat.cols);
+    ODL_REQUIRE(s.bytes <= workspace_bytes, "%s: workspace of %zu bytes needed for %d of [%lld, %lld], got %zu", who, s.bytes, count, (long long)mat.rows,
+                (long long)mat.cols, workspace_bytes);
     const bool tall  = mat.rows > mat.cols;
     const int64_t m = std::min(mat.rows, mat.cols), n = std::max(mat.rows, mat.cols), mp = padded(m), np = padded(n);
     const int parts = norm_blocks(mat.rows * mat.cols);
@@ -304,7 +308,8 @@ extern "C" size_t odl_hip_newton_schulz_workspace_bytes(int64_t batch, int64_t r
 {
     if (batch <= 0 || rows <= 0 || cols <= 0 || rows > kMostSide || cols > kMostSide)
         return 0;
-    return space_for(nullptr, group_of((int)std::min<int64_t>(batch, kGroup), rows, cols), rows, cols).bytes;
+    const int group = group_of((int)std::min<int64_t>(batch, kGroup), rows, cols), rest = (int)(batch % group);
+    return std::max(space_for(nullptr, group, rows, cols).bytes, rest ? space_for(nullptr, rest, rows, cols).bytes : (size_t)0);
 }
 
 extern "C" int odl_hip_newton_schulz(const float *g, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c, float eps, float *out,
@@ -329,7 +334,7 @@ extern "C" int odl_hip_newton_schulz(const float *g, int64_t batch, int64_t rows
         mat.rows = rows, mat.cols = cols;
         for (int i = 0; i < count; ++i)
             mat.g[i] = g + (first + i) * rows * cols, mat.out[i] = out + (first + i) * rows * cols;
-        if (int rc = run_group(mat, count, steps, a, b, c, eps, 1.f, 1.f, static_cast<char *>(workspace), odl::as_stream(stream)))
+        if (int rc = run_group(who, mat, count, steps, a, b, c, eps, 1.f, 1.f, workspace, workspace_bytes, odl::as_stream(stream)))
             return rc;
     }
     return ODL_OK;
@@ -397,7 +402,7 @@ extern "C" int odl_hip_muon_step_multi(int count, const float *const *p, const f
             mat.g[in] = g[j], mat.buf[in] = buf[j], mat.p[in] = p[j], mat.out[in] = p_out[j], ++in, --equal;
             if (in == group || equal == 0)
             {
-                if (int rc = run_group(mat, in, steps, a, b, c, eps, 1.f - lr * weight_decay, rate, static_cast<char *>(workspace), odl::as_stream(stream)))
+                if (int rc = run_group(who, mat, in, steps, a, b, c, eps, 1.f - lr * weight_decay, rate, workspace, workspace_bytes, odl::as_stream(stream)))
                     return rc;
                 in = 0;
             }
