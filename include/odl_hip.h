@@ -670,7 +670,9 @@ int odl_hip_sgd_step_multi_decay(int count, const float *const *p, float *const 
  * muon_step_multi: one optimiser step over a list of matrices [host_rows[i], host_cols[i]]; equal shapes go through the same
  * launches, up to 32 together:
  *   buf = momentum * buf + g;  u = nesterov ? g + momentum * buf : buf;  O = newton_schulz(u)
- *   p_out = p * (1 - lr * weight_decay) - lr * sqrt(max(1, rows / cols)) * O
+ *   p_out = p * (1 - lr * weight_decay) - lr * sqrt(max(1, outputs / inputs)) * O
+ * A matrix is [outputs, inputs] (a convolution's filters as [OC, the rest], LinearOp's weight); with host_in_out[i] != 0 in
+ * muon_step_multi_in_out entry i is [inputs, outputs], as nn::Linear keeps its weight (host_in_out null: none is).
  * buf is updated in place, p_out may be p; a buf or a p_out that stands for two entries is refused. Empty matrices are skipped.
  * Sides up to 2^20, 1 to 100 steps. Neither call synchronises or allocates device memory; both can be captured. */
 int odl_hip_newton_schulz(const float *g, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c,
@@ -680,6 +682,10 @@ int odl_hip_muon_step_multi(int count, const float *const *p, const float *const
                             const int64_t *host_cols, float lr, float momentum, int nesterov, float weight_decay, int steps,
                             float a, float b, float c, float eps, float *const *p_out, void *workspace, size_t workspace_bytes,
                             void *stream);
+int odl_hip_muon_step_multi_in_out(int count, const float *const *p, const float *const *g, float *const *buf, const int64_t *host_rows,
+                                   const int64_t *host_cols, const int *host_in_out, float lr, float momentum, int nesterov,
+                                   float weight_decay, int steps, float a, float b, float c, float eps, float *const *p_out,
+                                   void *workspace, size_t workspace_bytes, void *stream);
 size_t odl_hip_muon_step_multi_workspace_bytes(int count, const int64_t *host_rows, const int64_t *host_cols);
 /* origin::cuda::{zeros,ones,full} (cuda/factory.cuh:23-50) */
 int odl_hip_fill(float *dst, int64_t n, float value, void *stream);

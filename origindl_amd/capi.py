@@ -1148,10 +1148,11 @@ def newton_schulz(g, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
 
 
 def muon_step_multi(ps, gs, bufs, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
-                    coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+                    coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, in_out=None):
     """One orthogonalised-momentum step over a list of matrices: bufs[i] = momentum * bufs[i] + gs[i] in place, returns the new
-    parameters p * (1 - lr * weight_decay) - lr * sqrt(max(1, rows / cols)) * newton_schulz(update)."""
-    if not (len(ps) == len(gs) == len(bufs)):
+    parameters p * (1 - lr * weight_decay) - lr * sqrt(max(1, outputs / inputs)) * newton_schulz(update). A matrix is
+    [outputs, inputs], or [inputs, outputs] where in_out[i] is true (nn::Linear's weight)."""
+    if not (len(ps) == len(gs) == len(bufs)) or (in_out is not None and len(in_out) != len(ps)):
         raise OdlInvalidArgument("muon_step_multi: lists of different lengths")
     if not ps:
         return []
@@ -1172,8 +1173,9 @@ def muon_step_multi(ps, gs, bufs, lr, momentum=0.95, nesterov=True, weight_decay
     with _on(device):
         outs = [torch.empty_like(p) for p in ps]
         ws, nb = _ws_like(ps[0], lib().query("odl_hip_muon_step_multi_workspace_bytes", n, rows, cols))
-        lib().call("odl_hip_muon_step_multi", n, _ptr_array(ps), _ptr_array(gs), _ptr_array(bufs), rows, cols, float(lr), float(momentum),
-                   int(nesterov), float(weight_decay), int(steps), a, b, c, float(eps), _ptr_array(outs), _p(ws), nb, _stream())
+        flags = (ctypes.c_int * n)(*[1 if f else 0 for f in in_out]) if in_out is not None else None
+        lib().call("odl_hip_muon_step_multi_in_out", n, _ptr_array(ps), _ptr_array(gs), _ptr_array(bufs), rows, cols, flags, float(lr),
+                   float(momentum), int(nesterov), float(weight_decay), int(steps), a, b, c, float(eps), _ptr_array(outs), _p(ws), nb, _stream())
     return outs
 
 

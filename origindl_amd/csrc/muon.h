@@ -20,6 +20,7 @@ struct Matrices  // one launch's matrices: all [rows, cols]
     float *buf[kGroup];    // null: U is the gradient itself
     const float *p[kGroup];
     float *out[kGroup];    // X, or the new parameter where p is not null
+    float rate[kGroup];    // what X is multiplied by before it is taken from the parameter
     int64_t rows, cols;
     float momentum;
     int nesterov;
@@ -95,14 +96,14 @@ __device__ inline void store_columns(const Panel &p, int64_t cb, int64_t rb, int
 
 // a lane's part of X, block (row block rb of m, column block cb of n) of matrix z after to_columns: stored, or applied to the
 // parameter
-__device__ inline void write_result(const Matrices &a, int z, f32x16 &c, int64_t rb, int64_t cb, int lane, float keep, float rate)
+__device__ inline void write_result(const Matrices &a, int z, f32x16 &c, int64_t rb, int64_t cb, int lane, float keep)
 {
     const bool tall = a.rows > a.cols;
     const int64_t m = tall ? a.cols : a.rows, n = tall ? a.rows : a.cols, col = cb * 32 + (lane & 31);
     if (col >= n)
         return;
     const int64_t row0 = rb * 32 + 8 * (lane >> 5), at0 = tall ? col * m + row0 : row0 * n + col, step = tall ? 1 : n;
-    const float *p = a.p[z];
+    const float *p = a.p[z], rate = a.rate[z];
     float *out = a.out[z];
     // all of the parameter's elements are under way before the first new one is stored (p may be out)
     if (p)
@@ -151,7 +152,7 @@ __device__ inline double sum_of_parts(const double *sums, int parts, double *scr
 struct Settings
 {
     int steps;
-    float a, b, c, eps, keep, rate;
+    float a, b, c, eps, keep;
 };
 
 bool slim_fits(int64_t rows, int64_t cols);

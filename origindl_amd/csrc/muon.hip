@@ -3,7 +3,7 @@
 //   X0 = U / (||U||_F + eps), transposed if it has more rows than columns (m <= n from here on)
 //   X <- a X + (b A + c A A) X,  A = X X^T        `steps` times
 //   U: the gradient; in the optimiser step the momentum buf <- mu buf + g, or g + mu buf (Nesterov)
-//   p <- p (1 - lr * weight_decay) - lr * sqrt(max(1, rows / cols)) * X
+//   p <- p (1 - lr * weight_decay) - lr * sqrt(max(1, outputs / inputs)) * X       [outputs, inputs] or [inputs, outputs]
 //
 // What bounds it: three products a step, 2m^2 n + 2m^3 + 2m^2 n operations, of which the two symmetric ones need only half of
 // their tiles. They run as three float16 products each (split_gemm.h); X, A and b A + c A A live only as operands of
@@ -151,7 +151,7 @@ struct LastEpilogue
     int64_t batch_bytes;
     float own, before;
     Matrices a;
-    float keep, rate;  // p * keep - X * rate
+    float keep;  // p * keep - X * rate
     template <class T, class Acc>
     __device__ void operator()(const T &t, Acc &acc) const
     {
@@ -166,7 +166,7 @@ struct LastEpilogue
                 const int64_t rb = t.row_block(mi), cb = t.col_block(ni);
                 to_columns(c);
                 combine(c, q, cb, rb, t.lane, own, before);
-                write_result(a, t.z, c, rb, cb, t.lane, keep, rate);
+                write_result(a, t.z, c, rb, cb, t.lane, keep);
             }
     }
 };
@@ -257,7 +257,7 @@ int check_common(const char *who, int64_t rows, int64_t cols, int steps, float a
     return ODL_OK;
 }
 
-int run_group(const char *who, const Matrices &mat, int count, int steps, float a, float b, float c, float eps, float keep, float rate, void *workspace,
+int run_group(const char *who, const Matrices &mat, int count, int steps, float a, float b, float c, float eps, float keep, void *workspace,
               size_t workspace_bytes, hipStream_t st)
 {
     const Space s = space_for(static_cast<char *>(workspace), count, mat.rows, mat.cols);
@@ -272,7 +272,7 @@ int run_group(const char *who, const Matrices &mat, int count, int steps, float 
         ODL_LAUNCH_CHECK();
     }
     if (slim_fits(mat.rows, mat.cols))
-        return slim_run(mat, count, Settings{steps, a, b, c, eps, keep, rate}, s.sums, parts, s.xr[0].base, st);
+        return slim_run(mat, count, Settings{steps, a, b, c, eps, keep}, s.sums, parts, s.xr[0].base, st);
     const int64_t rp = tall ? np : mp, cp = tall ? mp : np;
     muon_prepare_kernel<<<dim3((unsigned)(cp / 64), (unsigned)(rp / 64), (unsigned)count), dim3(kBlock), 0, st>>>(
         mat, s.sums, parts, (double)eps, tall ? s.xt[0] : s.xr[0], tall ? s.xr[0] : s.xt[0], s.batch_bytes);
@@ -296,7 +296,7 @@ int run_group(const char *who, const Matrices &mat, int count, int steps, float 
         if (k + 1 < steps)
             rc = launch_whole_gemm(g, mp, np, s.step, s.parts, StepEpilogue{xt, s.xt[(k + 1) & 1], s.xr[(k + 1) & 1], s.batch_bytes, 1.f / kScale, a}, st);
         else
-            rc = launch_whole_gemm(g, mp, np, s.step, s.parts, LastEpilogue{xt, s.batch_bytes, 1.f / kScale / kScale, a / kScale, mat, keep, rate}, st);
+            rc = launch_whole_gemm(g, mp, np, s.step, s.parts, LastEpilogue{xt, s.batch_bytes, 1.f / kScale / kScale, a / kScale, mat, keep}, st);
         if (rc)
             return rc;
     }
@@ -334,7 +334,7 @@ extern "C" int odl_hip_newton_schulz(const float *g, int64_t batch, int64_t rows
         mat.rows = rows, mat.cols = cols;
         for (int i = 0; i < count; ++i)
             mat.g[i] = g + (first + i) * rows * cols, mat.out[i] = out + (first + i) * rows * cols;
-        if (int rc = run_group(who, mat, count, steps, a, b, c, eps, 1.f, 1.f, workspace, workspace_bytes, odl::as_stream(stream)))
+        if (int rc = run_group(who, mat, count, steps, a, b, c, eps, 1.f, workspace, workspace_bytes, odl::as_stream(stream)))
             return rc;
     }
     return ODL_OK;
@@ -356,6 +356,15 @@ extern "C" size_t odl_hip_muon_step_multi_workspace_bytes(int count, const int64
 extern "C" int odl_hip_muon_step_multi(int count, const float *const *p, const float *const *g, float *const *buf, const int64_t *host_rows,
                                        const int64_t *host_cols, float lr, float momentum, int nesterov, float weight_decay, int steps, float a, float b,
                                        float c, float eps, float *const *p_out, void *workspace, size_t workspace_bytes, void *stream)
+{
+    return odl_hip_muon_step_multi_in_out(count, p, g, buf, host_rows, host_cols, nullptr, lr, momentum, nesterov, weight_decay, steps, a, b, c, eps, p_out,
+                                          workspace, workspace_bytes, stream);
+}
+
+extern "C" int odl_hip_muon_step_multi_in_out(int count, const float *const *p, const float *const *g, float *const *buf, const int64_t *host_rows,
+                                              const int64_t *host_cols, const int *host_in_out, float lr, float momentum, int nesterov, float weight_decay,
+                                              int steps, float a, float b, float c, float eps, float *const *p_out, void *workspace,
+                                              size_t workspace_bytes, void *stream)
 {
     const char *who = "muon_step_multi";
     ODL_REQUIRE(count >= 0, "%s: negative count", who);
@@ -391,7 +400,6 @@ extern "C" int odl_hip_muon_step_multi(int count, const float *const *p, const f
         for (int j = i; j < count; ++j)
             equal += host_rows[j] == rows && host_cols[j] == cols;
         const int group = group_of(std::min(equal, kGroup), rows, cols);
-        const float rate = lr * (float)std::sqrt(std::max(1.0, (double)rows / (double)cols));
         Matrices mat{};
         mat.rows = rows, mat.cols = cols, mat.momentum = momentum, mat.nesterov = nesterov;
         int in = 0;
@@ -399,10 +407,13 @@ extern "C" int odl_hip_muon_step_multi(int count, const float *const *p, const f
         {
             if (host_rows[j] != rows || host_cols[j] != cols)
                 continue;
-            mat.g[in] = g[j], mat.buf[in] = buf[j], mat.p[in] = p[j], mat.out[in] = p_out[j], ++in, --equal;
+            mat.g[in] = g[j], mat.buf[in] = buf[j], mat.p[in] = p[j], mat.out[in] = p_out[j];
+            const bool in_out = host_in_out && host_in_out[j];
+            mat.rate[in] = lr * (float)std::sqrt(std::max(1.0, in_out ? (double)cols / (double)rows : (double)rows / (double)cols));
+            ++in, --equal;
             if (in == group || equal == 0)
             {
-                if (int rc = run_group(who, mat, in, steps, a, b, c, eps, 1.f - lr * weight_decay, rate, workspace, workspace_bytes, odl::as_stream(stream)))
+                if (int rc = run_group(who, mat, in, steps, a, b, c, eps, 1.f - lr * weight_decay, workspace, workspace_bytes, odl::as_stream(stream)))
                     return rc;
                 in = 0;
             }

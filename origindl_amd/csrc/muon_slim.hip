@@ -33,7 +33,7 @@ struct SlimArgs
     const f32x4 *share_in;
     f32x4 *share_out;
     int strips;
-    float ca, cb, cc, keep, rate;
+    float ca, cb, cc, keep;
 };
 
 enum
@@ -308,7 +308,7 @@ __global__ __launch_bounds__(MB == 4 ? 512 : 256, 2) void muon_slim_kernel(const
 #pragma unroll
                     for (int e = 0; e < 16; ++e)
                         x[i][e] *= 1.f / kScale;
-                    write_result(s.a, z, x[i], rb, rb0 + cb0 + i, lane, s.keep, s.rate);
+                    write_result(s.a, z, x[i], rb, rb0 + cb0 + i, lane, s.keep);
                 }
                 return;
             }
@@ -401,7 +401,7 @@ int slim_run(const Matrices &mat, int count, const Settings &set, const double *
     SlimArgs s{};
     s.a = mat, s.sums = sums, s.parts = parts, s.steps = set.steps, s.eps = (double)set.eps;
     s.xt = workspace, s.xt_bytes = sh.xt_bytes, s.strips = sh.strips;
-    s.ca = set.a, s.cb = set.b, s.cc = set.c, s.keep = set.keep, s.rate = set.rate;
+    s.ca = set.a, s.cb = set.b, s.cc = set.c, s.keep = set.keep;
     char *shares[2] = {workspace + count * sh.xt_bytes, workspace + count * (sh.xt_bytes + sh.share_bytes)};
     const dim3 grid((unsigned)sh.strips, (unsigned)count);
     const bool whole = slim_whole(mat.rows, mat.cols);

@@ -518,6 +518,7 @@ public:
     {
         const Mat *param, *grad;
         Mat *momentum;
+        bool inputs_first;  // [inputs, outputs], not [outputs, the rest]
     };
     static std::vector<std::unique_ptr<Mat>> muon_step_multi(const std::vector<MuonItem> &items, float lr, float momentum, bool nesterov,
                                                              float weight_decay, int steps, const float coefficients[3], float eps,

@@ -277,7 +277,9 @@ public:
 // Momentum whose direction is orthogonalised before it is applied, for a model's matrices; Adam for what is none. A matrix is
 // a parameter of two or more dimensions seen as [dim 0, the rest] with both larger than 1: a Linear's weight, a Conv2d's
 // filters, not a bias [1, out]. Per matrix: buf = momentum*buf + g; u = nesterov ? g + momentum*buf : buf;
-//   p = p*(1 - lr*weight_decay) - lr*sqrt(max(1, rows/cols)) * newton_schulz(u)
+//   p = p*(1 - lr*weight_decay) - lr*sqrt(max(1, outputs/inputs)) * newton_schulz(u)
+// where dim 0 counts the outputs, or the inputs of a Parameter that says so (inputs_first): a Linear's weight does, a module of
+// one's own says it of a weight [in, out] with set_inputs_first.
 // Matrices of equal shape go through the same launches; a parameter registered twice is stepped once. Settings are checked when the first step runs.
 struct MuonOptions
 {

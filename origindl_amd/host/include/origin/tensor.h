@@ -202,6 +202,15 @@ public:
         static_cast<Tensor &>(*this) = t;
         return *this;
     }
+    // Whether dim 0 counts a layer's inputs, as in nn::Linear's weight [in, out], and not its outputs, as in Conv2d's filters.
+    // A property of the layer's place for the value: assigning another value leaves it.
+    bool inputs_first() const { return inputs_first_; }
+    void set_inputs_first(bool yes) { inputs_first_ = yes; }
+    Parameter(const Parameter &) = default;
+    Parameter &operator=(const Parameter &p) { return *this = static_cast<const Tensor &>(p); }
+
+private:
+    bool inputs_first_ = false;
 };
 
 class Operator : public std::enable_shared_from_this<Operator>

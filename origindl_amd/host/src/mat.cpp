@@ -2328,9 +2328,11 @@ std::vector<std::unique_ptr<Mat>> OriginMat::muon_step_multi(const std::vector<M
     std::vector<const float *> p(count), g(count);
     std::vector<float *> buf(count), out(count);
     std::vector<int64_t> rows(count), cols(count);
+    std::vector<int> in_out(count);
     std::vector<std::unique_ptr<Mat>> results;
     for (size_t i = 0; i < count; ++i)
     {
+        in_out[i]           = items[i].inputs_first;
         const OriginMat &pm = dev_f32(*items[i].param, who), &gm = dev_f32(*items[i].grad, who), &bm = dev_f32(*items[i].momentum, who);
         if (gm.shape() != pm.shape() || bm.shape() != pm.shape() || pm.shape().size() < 2)
             THROW_INVALID_ARG("muon_step: parameter, gradient and momentum must have one shape of two or more dimensions, but got {} {} {}",
@@ -2349,8 +2351,9 @@ std::vector<std::unique_ptr<Mat>> OriginMat::muon_step_multi(const std::vector<M
     if (count == 0)
         return results;
     Workspace ws(odl_hip_muon_step_multi_workspace_bytes((int)count, rows.data(), cols.data()), items[0].param->device().index());
-    check(odl_hip_muon_step_multi((int)count, p.data(), g.data(), buf.data(), rows.data(), cols.data(), lr, momentum, nesterov, weight_decay,
-                                  steps, coefficients[0], coefficients[1], coefficients[2], eps, out.data(), ws.ptr(), ws.bytes, cur()));
+    check(odl_hip_muon_step_multi_in_out((int)count, p.data(), g.data(), buf.data(), rows.data(), cols.data(), in_out.data(), lr, momentum,
+                                         nesterov, weight_decay, steps, coefficients[0], coefficients[1], coefficients[2], eps, out.data(),
+                                         ws.ptr(), ws.bytes, cur()));
     return results;
 }
 

@@ -268,6 +268,7 @@ Linear::Linear(int in_features, int out_features, bool bias)
     : in_features_(in_features), out_features_(out_features), use_bias_(bias)
 {
     reset_parameters();
+    weight_.set_inputs_first(true);
     register_parameter("weight", weight_);
     if (use_bias_)
         register_parameter("bias", bias_);
@@ -701,7 +702,7 @@ void Muon::step_all(std::vector<Parameter *> &params)
                 THROW_RUNTIME_ERROR("Muon: run one ordinary step before capturing (the momentum buffers must exist)");
             momentum_buffers_.emplace(p, Tensor::zeros(grad.shape(), TensorOptions(grad.dtype()).device(grad.device())));
         }
-        items.push_back({p->impl_->data_.get(), grad.impl_->data_.get(), momentum_buffers_.at(p).impl_->data_.get()});
+        items.push_back({p->impl_->data_.get(), grad.impl_->data_.get(), momentum_buffers_.at(p).impl_->data_.get(), p->inputs_first()});
     }
     const float coefficients[3] = {options_.a, options_.b, options_.c};
     auto updated = OriginMat::muon_step_multi(items, lr_, options_.momentum, options_.nesterov, options_.weight_decay, options_.steps,

@@ -1725,5 +1725,47 @@ int DRV(muon_shared)(const float *p, const float *g, int64_t rows, int64_t cols,
         out(std::any_cast<Module::StateDict>(state.at("momentum_buffers")).begin()->second, kept);
     });
 }
+
+// One Muon step of a parameter [rows, cols] (filters: [rows, cols / 4, 2, 2]) with the gradient g. kind 0: a module's own parameter;
+// 1: one it calls inputs-first; 2: a Linear's weight, after a value has been assigned to it; 3: a Conv2d's filters
+int DRV(muon_place)(const float *p, const float *g, int64_t rows, int64_t cols, int kind, float lr, float *o)
+{
+    return guarded([&] {
+        struct Holder : Module
+        {
+            Parameter p;
+            Holder(const Tensor &t, bool inputs_first) : p(t)
+            {
+                p.set_inputs_first(inputs_first);
+                register_parameter("p", p);
+            }
+            Tensor forward(const Tensor &x) override { return x; }
+        };
+        const Shape shape = kind == 3 ? Shape{(size_t)rows, (size_t)(cols / 4), 2, 2} : Shape{(size_t)rows, (size_t)cols};
+        std::unique_ptr<Module> model;
+        Parameter *q;
+        if (kind == 2)
+        {
+            auto l = std::make_unique<nn::Linear>((int)rows, (int)cols, false);
+            q = l->weight(), model = std::move(l);
+        }
+        else if (kind == 3)
+        {
+            auto c = std::make_unique<nn::Conv2d>((int)cols / 4, (int)rows, 2, 1, 0, false);
+            q = c->weight(), model = std::move(c);
+        }
+        else
+        {
+            auto h = std::make_unique<Holder>(f32(p, shape, true), kind == 1);
+            q = &h->p, model = std::move(h);
+        }
+        *q = Parameter(f32(p, shape, true));
+        Muon opt(*model, lr);
+        auto G = f32(g, shape);
+        F::sum(*q * G).backward();
+        opt.step();
+        out(*q, o);
+    });
+}
 #endif
 }  // extern "C"

@@ -126,6 +126,7 @@ _DEVICE_ONLY_SIGS = {
     "odl_host_newton_schulz": "plllip>i",
     "odl_host_muon_train": "ppllll" "iifffpp>i",
     "odl_host_muon_shared": "ppllii" "fpp>i",
+    "odl_host_muon_place": "ppllif" "p>i",
 }
 
 

@@ -32,3 +32,92 @@ def test_a_batch_stays_inside_the_workspace_it_asks_for(capi, count, rows, cols)
     for i in (0, 31, 32, count - 1):
         want = schulz64(g[i])
         assert float((out[i].double() - want).norm()) <= schulz_bar(5) * max(1.0, float(want.norm())), i
+
+
+# ---------------------------------------------------------------------------------- the factor of an update: outputs and inputs
+def factor(inputs, outputs):
+    """What an orthogonalised update of a layer is multiplied by: more where it has more outputs than inputs."""
+    return math.sqrt(max(1.0, outputs / inputs))
+
+
+@pytest.fixture(scope="module")
+def h():
+    import oraclelib as ol
+    return ol.host_driver()
+
+
+def muon_of(p, g, buf, lr, scale, decay=0.0, momentum=0.95):
+    buf = momentum * buf + g
+    o = schulz64(g + momentum * buf)
+    return p * (1 - lr * decay) - lr * scale * o, buf, lr * scale * float(o.norm())
+
+
+def test_updates_of_matrices_kept_either_way_round(capi):
+    """[outputs, inputs], [inputs, outputs] and both of one shape in the same launches."""
+    shapes = [(96, 40), (96, 40), (40, 96), (40, 96), (300, 130), (300, 130), (200, 4100), (4100, 200), (70, 70)]
+    in_out = [False, True, False, True, True, False, True, True, True]
+    g = gen(51)
+    ps, gs, bufs = ([torch.randn(*s, device="cuda", generator=g) for s in shapes] for _ in range(3))
+    want = [muon_of(p.double(), q.double(), b.double(), 0.05, factor(*(s if f else s[::-1])), 0.1)
+            for p, q, b, s, f in zip(ps, gs, bufs, shapes, in_out)]
+    new = capi.muon_step_multi(ps, gs, [b.clone() for b in bufs], lr=0.05, weight_decay=0.1, in_out=in_out)
+    for p, n, (w, _, unit) in zip(ps, new, want):
+        assert float((n.double() - w).norm()) <= schulz_bar(5) * unit + 2.0 ** -22 * float(p.norm())
+    # without the list all are [outputs, inputs]
+    plain = capi.muon_step_multi(ps, gs, [b.clone() for b in bufs], lr=0.05, weight_decay=0.1)
+    none = capi.muon_step_multi(ps, gs, [b.clone() for b in bufs], lr=0.05, weight_decay=0.1, in_out=[False] * len(ps))
+    assert all(torch.equal(a, b) for a, b in zip(plain, none))
+    assert all(torch.equal(a, b) for a, b, f in zip(plain, new, in_out) if not f)
+    with pytest.raises(capi.OdlInvalidArgument):
+        capi.muon_step_multi(ps, gs, bufs, lr=0.05, in_out=[True])
+
+
+@pytest.mark.parametrize("rows,cols", [(40, 96), (96, 40)])
+@pytest.mark.parametrize("kind", [0, 1, 2, 3])
+def test_host_optimizer_knows_which_side_counts_the_outputs(h, rows, cols, kind):
+    g = torch.Generator().manual_seed(52)
+    p, q = torch.randn(rows, cols, generator=g), torch.randn(rows, cols, generator=g)
+    o = np.empty((rows, cols), np.float32)
+    assert h.odl_host_muon_place(p.numpy(), q.numpy(), rows, cols, kind, 0.05, o) == 0
+    scale = factor(rows, cols) if kind in (1, 2) else factor(cols, rows)
+    want, _, unit = muon_of(p.double(), q.double(), torch.zeros(rows, cols, dtype=torch.float64), 0.05, scale)
+    assert float((torch.from_numpy(o).double() - want).norm()) <= schulz_bar(5) * unit + 2.0 ** -22 * float(p.norm())
+
+
+def test_training_steps_with_muon(h):
+    """Linear, ReLU, Linear and the loss, the weights by Muon and the biases by Adam: three steps, of them the last recorded or with
+    the state moved into a fresh optimizer, give the bits of plain ones; the first one is held to 64 bits. An orthogonalised
+    update's elements err by its bar, its inputs' error (relative 1e-5) passes through five steps with at most 3.4445 each."""
+    N, D, H, V, lr, decay, adam_lr = 48, 40, 72, 300, 0.02, 0.01, 1e-3
+    g = torch.Generator().manual_seed(41)
+    x, t = torch.randn(N, D, generator=g), torch.randint(0, V, (N,), generator=g)
+    start = [torch.randn(D, H, generator=g) / D ** 0.5, 0.1 * torch.randn(1, H, generator=g), torch.randn(H, V, generator=g) / H ** 0.5,
+             0.1 * torch.randn(1, V, generator=g)]
+    flat = torch.cat([p.reshape(-1) for p in start]).numpy()
+    results = []
+    for mode in (0, 1, 2):
+        params, losses = flat.copy(), np.zeros(3, np.float32)
+        assert h.odl_host_muon_train(x.numpy(), t.numpy(), N, D, H, V, 3, mode, lr, decay, adam_lr, params, losses) == 0
+        results.append((params, losses))
+    for params, losses in results[1:]:
+        assert np.array_equal(params, results[0][0]) and np.array_equal(losses, results[0][1])
+    params, losses = flat.copy(), np.zeros(1, np.float32)
+    assert h.odl_host_muon_train(x.numpy(), t.numpy(), N, D, H, V, 1, 0, lr, decay, adam_lr, params, losses) == 0
+    w1, b1, w2, b2 = (p.double().cuda() for p in start)
+    pre = x.double().cuda() @ w1 + b1
+    (loss, ga, gw2, gb2), _ = definition(pre.clamp(min=0), w2, b2, t.cuda(), False)
+    gp = ga * (pre > 0)
+    zero = torch.zeros((), dtype=torch.float64, device="cuda")
+    assert abs(float(losses[0]) - float(loss)) <= 1e-4 * float(loss)
+    at = 0
+    for p, w, grad in ((start[0], w1, x.double().cuda().t() @ gp), (start[1], b1, gp.sum(0)), (start[2], w2, gw2), (start[3], b2, gb2)):
+        got = torch.from_numpy(params[at:at + p.numel()]).reshape(p.shape).cuda().double()
+        at += p.numel()
+        if p.shape[0] > 1:
+            want, _, unit = muon_of(w, grad, zero, lr, factor(*p.shape), decay)
+            assert float((got - want).norm()) <= unit * (schulz_bar(5) + 1e-5 * 3.4445 ** 5) + 2.0 ** -22 * float(p.norm())
+        else:
+            # Adam's first step is adam_lr * g / (|g| + 1e-8): the sign, where the gradient is known well enough
+            sure = grad.reshape(p.shape).abs() > 1e-4 * grad.abs().max()
+            want = w - adam_lr * grad.reshape(p.shape) / (grad.reshape(p.shape).abs() + 1e-8)
+            assert bool(((got - want).abs()[sure] <= 0.01 * adam_lr).all()) and bool(((got - w).abs() <= 1.01 * adam_lr).all())
