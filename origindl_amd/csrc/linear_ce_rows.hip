@@ -5,7 +5,8 @@
 //   forward    one pass: logits of 128 (64) entries a workgroup, their maximum and sum of powers in its epilogue
 //   backward   the logits, which the forward pass has kept if they are small beside the weights (else one pass for them again):
 //              the same epilogue in both cases writes d = softmax - one-hot (the weights' size times 3N / K) and gb; one pass for
-//              gx = d.w, in runs of the vocabulary; gw = d^T.x writes its size once.
+//              gx = d.w, in runs of the vocabulary; gw = d^T.x writes its size once. d takes 12 bytes a row and entry: beyond
+//              512 MB of it the vocabulary goes through in pieces, whose sums for gx add up.
 //
 // Mathematics. A float32 number is the sum of three bfloat16 numbers, its first, second and third eight bits, cut off without
 // rounding: exact. Of the nine products of two such sums the six of at least 2^-16 of the whole are formed by bfloat16 matrix
@@ -366,13 +367,13 @@ struct RowsStatsEpilogue
     }
 };
 
-// d split: by_n as the small operand of gx, [V / 16][blocks of 32 rows]; by_v as an operand of gw, rows of the vocabulary, [V / 32][rows
-// / 16] (null: not wanted); and the sums over this workgroup's rows for gb
+// d of a piece of the vocabulary, split: by_n as the small operand of gx, [V / 16][blocks of 32 rows]; by_v as an operand of gw, rows
+// of the vocabulary, [V / 32][rows / 16] (null: not wanted); and the sums over this workgroup's rows for gb
 struct RowsGradEpilogue
 {
     const float *b, *saved, *row;
     Labels labels;
-    int64_t V;
+    int64_t v0, V;  // the piece's first entry, and how many it has
     u32x4 *by_n, *by_v;
     float *sums;  // [V padded to tiles][workgroups of rows]
     template <int VB, int NB, bool OUT_ROWS>
@@ -403,7 +404,7 @@ struct RowsGradEpilogue
                     if (counts && v < V)
                     {
                         d = pow2(fmaf(z[nb][e] + bias[e], kLog2e, -m2)) * inv;
-                        if (v == label)
+                        if (v == label - v0)
                             d -= 1.f;
                     }
                     lds[at * kPitch + nb * 32 + (lane & 31)] = d;
@@ -476,11 +477,12 @@ __global__ __launch_bounds__(64 * kWaves) void ce_kept_kernel(const float *__res
     epilogue.template run<VB, NB, OUT_ROWS>(tile, nb0, blocks_n, wave, lane, sum, lds);
 }
 
-// parts[run][feature][rows]
+// parts[run][feature][rows], (+)= over the pieces of the vocabulary
 struct RowsPartEpilogue
 {
     float *parts;
     int64_t outs;
+    int add;
     template <int VB, int NB, bool OUT_ROWS>
     __device__ void run(int64_t tile, int nb0, int blocks_n, int m, int lane, f32x16 *z, float *) const
     {
@@ -493,7 +495,10 @@ struct RowsPartEpilogue
             {
                 const int64_t o = tile * (32 * VB) + place_of<VB, OUT_ROWS>(m, lane, e);
                 if (o < outs)
-                    parts[((int64_t)blockIdx.y * outs + o) * (blocks_n * 32) + (nb0 + nb) * 32 + (lane & 31)] = z[nb][e];
+                {
+                    float *at = parts + ((int64_t)blockIdx.y * outs + o) * (blocks_n * 32) + (nb0 + nb) * 32 + (lane & 31);
+                    *at       = add ? *at + z[nb][e] : z[nb][e];
+                }
             }
     }
 };
@@ -537,7 +542,7 @@ __global__ __launch_bounds__(kBlock) void ce_rows_gx_kernel(const float *__restr
 
 // gw = factor * d^T.x over the rows: out[r][c] from operands split by r and by c, [blocks of 32][rows / 16]. A wave makes 32 rows of 128
 // columns; the four waves of a workgroup share the columns' operand, and walk down `steps` blocks of 128 rows.
-__global__ __launch_bounds__(kBlock, 2) void ce_rows_outer_kernel(const u32x4 *__restrict__ by_r, const u32x4 *__restrict__ by_c, int kbs, int64_t rows, int64_t cols,
+__global__ __launch_bounds__(kBlock, 2) void ce_rows_outer_kernel(const u32x4 *__restrict__ by_r, const u32x4 *__restrict__ by_c, int kbs, int64_t rows, int64_t cols, int64_t ld,
                                                                   unsigned tiles_c, int steps, const float *saved, const float *gy, float *__restrict__ out)
 {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -583,7 +588,7 @@ __global__ __launch_bounds__(kBlock, 2) void ce_rows_outer_kernel(const u32x4 *_
             {
                 const int64_t row = r0 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
                 if (row < rows)
-                    out[row * cols + col] = acc[m][e] * g;
+                    out[row * ld + col] = acc[m][e] * g;
             }
         }
     }
@@ -608,6 +613,13 @@ int64_t tile_of(int blocks_n)
 size_t fragments_bytes(int64_t rows, int64_t blocks_n)
 {
     return (size_t)odl::ceil_div(rows, 128) * 8 * (size_t)blocks_n * kFragment * 16;
+}
+
+// Entries of the vocabulary whose d, as both operands of its products, stays within 512 MB: whole tiles, in equal pieces.
+int64_t piece_of(int64_t V, int blocks_n)
+{
+    const int64_t most = ((int64_t)1 << 29) / (2 * 6 * 32 * blocks_n) / 128 * 128, pieces = odl::ceil_div(V, most);
+    return pieces == 1 ? V : odl::ceil_div(odl::ceil_div(V, pieces), 128) * 128;
 }
 
 int runs_for_gx(int64_t K, int64_t V, int blocks_n)
@@ -643,13 +655,14 @@ FewSpace backward_space(char *base, int64_t N, int64_t K, int64_t V)
 {
     FewSpace s{};
     Carver c{base};
-    const int blocks_n = blocks_of(N);
+    const int blocks_n  = blocks_of(N);
+    const int64_t piece = piece_of(V, blocks_n);
     s.x_by_n = c.take<u32x4>(fragments_bytes(K, blocks_n));
     s.x_by_k = c.take<u32x4>(fragments_bytes(K, blocks_n));
-    s.d_by_n = c.take<u32x4>(fragments_bytes(V, blocks_n));
-    s.d_by_v = c.take<u32x4>(fragments_bytes(V, blocks_n));
-    s.sums   = c.take<float>((size_t)odl::ceil_div(V, 128) * 128 * 2 * 4);
-    s.parts  = c.take<float>((size_t)runs_for_gx(K, V, blocks_n) * (size_t)K * (size_t)blocks_n * 32 * 4);
+    s.d_by_n = c.take<u32x4>(fragments_bytes(piece, blocks_n));
+    s.d_by_v = c.take<u32x4>(fragments_bytes(piece, blocks_n));
+    s.sums   = c.take<float>((size_t)odl::ceil_div(piece, 128) * 128 * 2 * 4);
+    s.parts  = c.take<float>((size_t)runs_for_gx(K, piece, blocks_n) * (size_t)K * (size_t)blocks_n * 32 * 4);
     s.bytes  = c.used;
     return s;
 }
@@ -748,34 +761,40 @@ int few_backward(const Problem &p, const float *gy, const float *saved, const fl
     if (gw || !kept)
         if (int rc = prepare(p, blocks_n, kept ? nullptr : s.x_by_n, gw ? s.x_by_k : nullptr, nullptr, st))
             return rc;
-    const int64_t ld = p.w_out_in ? p.K : p.V;
-    const RowsGradEpilogue e{p.b, saved, row_stats, p.labels, p.V, gx ? s.d_by_n : nullptr, gw ? s.d_by_v : nullptr, gb ? s.sums : nullptr};
-    if (int rc = kept ? from_kept(row_stats + 2 * p.N, p.w_out_in != 0, p.V, blocks_n, e, st)
-                      : stream(p.w, p.w_out_in != 0, ld, p.V, p.K, s.x_by_n, blocks_n, 1, e, st))
-        return rc;
-    if (gb)
+    const int64_t ld = p.w_out_in ? p.K : p.V, piece = piece_of(p.V, blocks_n);
+    const int runs = runs_for_gx(p.K, piece, blocks_n);
+    for (int64_t v0 = 0; v0 < p.V; v0 += piece)
     {
-        ce_rows_gb_kernel<<<dim3((unsigned)ceil_div(p.V, kBlock)), dim3(kBlock), 0, st>>>(s.sums, blocks_n / taken_of(blocks_n), p.V, saved, gy, gb);
-        ODL_LAUNCH_CHECK();
+        const int64_t vn = std::min(piece, p.V - v0), at = v0 * (p.w_out_in ? p.K : 1);
+        const RowsGradEpilogue e{p.b ? p.b + v0 : nullptr, saved, row_stats, p.labels, v0, vn, gx ? s.d_by_n : nullptr, gw ? s.d_by_v : nullptr,
+                                 gb ? s.sums : nullptr};
+        if (int rc = kept ? from_kept(row_stats + 2 * p.N + v0 * (blocks_n * 32), p.w_out_in != 0, vn, blocks_n, e, st)
+                          : stream(p.w + at, p.w_out_in != 0, ld, vn, p.K, s.x_by_n, blocks_n, 1, e, st))
+            return rc;
+        if (gb)
+        {
+            ce_rows_gb_kernel<<<dim3((unsigned)ceil_div(vn, kBlock)), dim3(kBlock), 0, st>>>(s.sums, blocks_n / taken_of(blocks_n), vn, saved, gy, gb + v0);
+            ODL_LAUNCH_CHECK();
+        }
+        if (gx)
+            if (int rc = stream(p.w + at, p.w_out_in == 0, ld, p.K, vn, s.d_by_n, blocks_n, runs, RowsPartEpilogue{s.parts, p.K, v0 > 0}, st))
+                return rc;
+        if (gw)
+        {
+            const int64_t r = p.w_out_in ? vn : p.K, c = p.w_out_in ? p.K : vn;
+            // enough workgroups for the chip, and as many rows each as that leaves: they share the columns' operand
+            const int64_t tiles_c = ceil_div(c, 128), tiles_r = ceil_div(r, 128);
+            const int steps = (int)std::max<int64_t>(1, std::min<int64_t>(16, tiles_c * tiles_r / (8 * (int64_t)device_cus())));
+            const int64_t blocks = tiles_c * ceil_div(tiles_r, steps);
+            ODL_REQUIRE(blocks < ((int64_t)1 << 31), "linear_softmax_ce: too many tiles");
+            ce_rows_outer_kernel<<<dim3((unsigned)blocks), dim3(kBlock), 0, st>>>(p.w_out_in ? s.d_by_v : s.x_by_k, p.w_out_in ? s.x_by_k : s.d_by_v,
+                                                                                 blocks_n * 2, r, c, ld, (unsigned)tiles_c, steps, saved, gy, gw + at);
+            ODL_LAUNCH_CHECK();
+        }
     }
     if (gx)
     {
-        const int runs = runs_for_gx(p.K, p.V, blocks_n);
-        if (int rc = stream(p.w, p.w_out_in == 0, ld, p.K, p.V, s.d_by_n, blocks_n, runs, RowsPartEpilogue{s.parts, p.K}, st))
-            return rc;
         ce_rows_gx_kernel<<<dim3((unsigned)ceil_div(p.K, 32), (unsigned)blocks_n), dim3(kBlock), 0, st>>>(s.parts, runs, p.N, p.K, blocks_n * 32, saved, gy, gx);
-        ODL_LAUNCH_CHECK();
-    }
-    if (gw)
-    {
-        const int64_t r = p.w_out_in ? p.V : p.K, c = p.w_out_in ? p.K : p.V;
-        // enough workgroups for the chip, and as many rows each as that leaves: they share the columns' operand
-        const int64_t tiles_c = ceil_div(c, 128), tiles_r = ceil_div(r, 128);
-        const int steps = (int)std::max<int64_t>(1, std::min<int64_t>(16, tiles_c * tiles_r / (8 * (int64_t)device_cus())));
-        const int64_t blocks = tiles_c * ceil_div(tiles_r, steps);
-        ODL_REQUIRE(blocks < ((int64_t)1 << 31), "linear_softmax_ce: too many tiles");
-        ce_rows_outer_kernel<<<dim3((unsigned)blocks), dim3(kBlock), 0, st>>>(p.w_out_in ? s.d_by_v : s.x_by_k, p.w_out_in ? s.x_by_k : s.d_by_v, blocks_n * 2, r, c,
-                                                                             (unsigned)tiles_c, steps, saved, gy, gw);
         ODL_LAUNCH_CHECK();
     }
     return ODL_OK;

@@ -121,3 +121,18 @@ def test_training_steps_with_muon(h):
             sure = grad.reshape(p.shape).abs() > 1e-4 * grad.abs().max()
             want = w - adam_lr * grad.reshape(p.shape) / (grad.reshape(p.shape).abs() + 1e-8)
             assert bool(((got - want).abs()[sure] <= 0.01 * adam_lr).all()) and bool(((got - w).abs() <= 1.01 * adam_lr).all())
+
+
+# ----------------------------------------------------------------------------------------------------- large vocabularies
+@pytest.mark.parametrize("shape", [(256, 33, 400001), (90, 40, 500000), (40, 130, 1600003), (3, 150, 1500001), (200, 1024, 200001)])
+@pytest.mark.parametrize("out_in", [False, True])
+def test_few_rows_over_a_vocabulary_in_several_pieces(capi, shape, out_in):
+    """Pieces that end inside a tile, with and without logits kept from the forward pass: gx adds up over them, gw and gb are written
+    piece by piece, a label may lie in any of them."""
+    N, K, V = shape
+    x, w, b, t = make(N, K, V, out_in, True, 0.1, True, seed=61)
+    t[0], t[N // 2], t[N - 1] = 0, V // 2, V - 1
+    got, saved = run(capi, x, w, b, t, out_in)
+    check(got, *definition(x, w, b, t, out_in))
+    part = capi.linear_softmax_cross_entropy_backward(None, x, w, b, t, saved, w_out_in=out_in, need_gw=False, need_gb=False)
+    assert torch.equal(part[0], got[1])

@@ -68,3 +68,14 @@ def test_a_workspace_for_the_full_group_alone_is_refused(l):
     coef = (3.4445, -4.7750, 2.0315)
     assert l.cdll.odl_hip_newton_schulz(some, count, rows, cols, 5, *coef, 1e-7, some, some, nb, None) == _lib.ODL_ERR_INVALID_ARG
     assert "workspace" in l.last_error()
+
+
+@pytest.mark.parametrize("N", [1, 32, 64, 128, 200, 256, 257, 4096])
+def test_backward_goes_over_the_vocabulary_in_pieces_whatever_the_rows(l, N):
+    """softmax - one-hot never lies in the workspace whole: what a call asks for has a bound in V."""
+    q = lambda K, V: l.query("odl_hip_linear_softmax_ce_backward_workspace_bytes", N, K, V)
+    for K in (1, 64, 1024):
+        sizes = [q(K, V) for V in (10_000_000, 100_000_000, 1 << 30)]
+        assert max(sizes) < 1 << 30, (K, sizes)
+        assert max(sizes) - min(sizes) < 64 << 20, (K, sizes)  # pieces of equal size, up to a tile
+    assert q(1024, 1_000_000) < 1 << 30
