@@ -516,6 +516,8 @@ Plan make_plan(int64_t N, int64_t K, int64_t V, bool backward)
     // backward: d twice and w twice, 4 bytes an element; forward: w once
     const int64_t budget = (int64_t)1 << 26;
     int64_t most = backward ? std::min(budget / p.n_pad, budget / p.k_pad) : budget / p.k_pad;
+    // a launch's threads have to fit 32 bits: one for 16 logits in the smallest tiles
+    most = std::min(most, ((int64_t)1 << 35) / p.n_pad);
     most = std::max<int64_t>(most / 256 * 256, 1024);
     p.pieces  = odl::ceil_div(V, most);
     p.v_piece = p.pieces == 1 ? V : odl::ceil_div(odl::ceil_div(V, p.pieces), 256) * 256;

@@ -305,7 +305,7 @@ struct RowsStatsEpilogue
 {
     const float *b;
     Labels labels;
-    int64_t V;
+    int64_t v0, V;  // the launch's first entry, and how many it has
     float *part_m, *part_s, *target;
     float *kept;  // null, or where x.w stays for the backward pass (rows past the batch are left out)
     template <int VB, int NB, bool OUT_ROWS>
@@ -324,7 +324,7 @@ struct RowsStatsEpilogue
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
             {
-                const int64_t n = (nb0 + nb) * 32 + (lane & 31), label = labels(n) - tile * (32 * VB);
+                const int64_t n = (nb0 + nb) * 32 + (lane & 31), label = labels(n) - v0 - tile * (32 * VB);
                 float top = -INFINITY;
                 if (kept && n < labels.N)
                 {
@@ -667,13 +667,21 @@ FewSpace backward_space(char *base, int64_t N, int64_t K, int64_t V)
     return s;
 }
 
+// a launch's threads along x have to fit 32 bits
+int check_blocks(int64_t blocks, int threads)
+{
+    ODL_REQUIRE(blocks <= ((int64_t)1 << 32) / threads - 1, "linear_softmax_ce: too many tiles");
+    return ODL_OK;
+}
+
 template <class Epilogue>
 int stream(const float *w, bool out_rows, int64_t ld, int64_t outs, int64_t contraction, const u32x4 *q, int blocks_n, int runs, const Epilogue &e, hipStream_t st)
 {
     Stream a{w, ld, outs, contraction, q, blocks_n, odl::ceil_div(contraction, 16), 0};
     a.wave_groups = odl::ceil_div(a.groups, (int64_t)runs * kWaves);
     const int64_t blocks = odl::ceil_div(outs, tile_of(blocks_n)) * (blocks_n / taken_of(blocks_n));
-    ODL_REQUIRE(blocks < ((int64_t)1 << 31), "linear_softmax_ce: too many tiles");
+    if (int rc = check_blocks(blocks, 64 * kWaves))
+        return rc;
     const dim3 grid((unsigned)blocks, (unsigned)runs), block(64 * kWaves);
     switch (taken_of(blocks_n) * 2 + (out_rows ? 1 : 0))
     {
@@ -692,7 +700,8 @@ template <class Epilogue>
 int from_kept(const float *kept, bool out_rows, int64_t outs, int blocks_n, const Epilogue &e, hipStream_t st)
 {
     const int64_t blocks = odl::ceil_div(outs, tile_of(blocks_n)) * (blocks_n / taken_of(blocks_n));
-    ODL_REQUIRE(blocks < ((int64_t)1 << 31), "linear_softmax_ce: too many tiles");
+    if (int rc = check_blocks(blocks, 64 * kWaves))
+        return rc;
     const dim3 grid((unsigned)blocks), block(64 * kWaves);
     switch (taken_of(blocks_n) * 2 + (out_rows ? 1 : 0))
     {
@@ -746,10 +755,17 @@ int few_forward(const Problem &p, float *saved, float *row_stats, char *workspac
     if (int rc = prepare(p, blocks_n, s.x_by_n, nullptr, saved, st))
         return rc;
     float *kept = few_kept_floats(p.N, p.K, p.V) ? row_stats + 2 * p.N : nullptr;
-    const RowsStatsEpilogue e{p.b, p.labels, p.V, s.part_m, s.part_s, s.target, kept};
-    if (int rc = stream(p.w, p.w_out_in != 0, p.w_out_in ? p.K : p.V, p.V, p.K, s.x_by_n, blocks_n, 1, e, st))
-        return rc;
-    return join(s.part_m, s.part_s, s.target, ceil_div(p.V, tile_of(blocks_n)), blocks_n * 32, p.labels, row_stats, s.join_scratch, saved, st);
+    // as many entries in a launch as its threads along x can be counted in 32 bits: 2^27 or more
+    const int64_t tile = tile_of(blocks_n), rows = blocks_n * 32, most = ((int64_t)1 << 22) / (blocks_n / taken_of(blocks_n)) * tile;
+    for (int64_t v0 = 0; v0 < p.V; v0 += most)
+    {
+        const int64_t vn = std::min(most, p.V - v0), at = v0 * (p.w_out_in ? p.K : 1);
+        const RowsStatsEpilogue e{p.b ? p.b + v0 : nullptr, p.labels, v0, vn, s.part_m + v0 / tile * rows, s.part_s + v0 / tile * rows, s.target,
+                                  kept ? kept + v0 * rows : nullptr};
+        if (int rc = stream(p.w + at, p.w_out_in != 0, p.w_out_in ? p.K : p.V, vn, p.K, s.x_by_n, blocks_n, 1, e, st))
+            return rc;
+    }
+    return join(s.part_m, s.part_s, s.target, ceil_div(p.V, tile), rows, p.labels, row_stats, s.join_scratch, saved, st);
 }
 
 int few_backward(const Problem &p, const float *gy, const float *saved, const float *row_stats, float *gx, float *gw, float *gb, char *workspace,
@@ -786,7 +802,8 @@ int few_backward(const Problem &p, const float *gy, const float *saved, const fl
             const int64_t tiles_c = ceil_div(c, 128), tiles_r = ceil_div(r, 128);
             const int steps = (int)std::max<int64_t>(1, std::min<int64_t>(16, tiles_c * tiles_r / (8 * (int64_t)device_cus())));
             const int64_t blocks = tiles_c * ceil_div(tiles_r, steps);
-            ODL_REQUIRE(blocks < ((int64_t)1 << 31), "linear_softmax_ce: too many tiles");
+            if (int rc = check_blocks(blocks, kBlock))
+                return rc;
             ce_rows_outer_kernel<<<dim3((unsigned)blocks), dim3(kBlock), 0, st>>>(p.w_out_in ? s.d_by_v : s.x_by_k, p.w_out_in ? s.x_by_k : s.d_by_v,
                                                                                  blocks_n * 2, r, c, ld, (unsigned)tiles_c, steps, saved, gy, gw + at);
             ODL_LAUNCH_CHECK();

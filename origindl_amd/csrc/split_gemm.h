@@ -596,7 +596,8 @@ template <class Epilogue>
 inline int launch_tiles(const GemmArgs &g, const Cut &cut, const Epilogue &e, hipStream_t st)
 {
     const int64_t blocks = g.blocks();
-    ODL_REQUIRE(blocks < ((int64_t)1 << 31), "product of too many tiles");
+    const int threads    = cut.bm * cut.bn > 128 * 128 ? 512 : 256;
+    ODL_REQUIRE(blocks <= ((int64_t)1 << 32) / threads - 1, "product of too many tiles");
     if (blocks == 0 || g.nkb == 0)
         return fail(ODL_ERR_RUNTIME, "empty product");
     const dim3 grid((unsigned)blocks);
@@ -640,7 +641,7 @@ inline int launch_whole_gemm(const GemmArgs &args, int64_t rows_pad, int64_t col
         return rc;
     g = cut_args(args, rows_pad, cols_pad, Cut{64, 64, 1, args.nkb});
     const int64_t blocks = g.blocks();
-    ODL_REQUIRE(blocks < ((int64_t)1 << 31), "product of too many tiles");
+    ODL_REQUIRE(blocks <= ((int64_t)1 << 32) / 256 - 1, "product of too many tiles");
     split_gemm_finish_kernel<Epilogue><<<dim3((unsigned)blocks), dim3(256), 0, st>>>(g, p, e);
     ODL_LAUNCH_CHECK();
     return ODL_OK;

@@ -136,3 +136,36 @@ def test_few_rows_over_a_vocabulary_in_several_pieces(capi, shape, out_in):
     check(got, *definition(x, w, b, t, out_in))
     part = capi.linear_softmax_cross_entropy_backward(None, x, w, b, t, saved, w_out_in=out_in, need_gw=False, need_gb=False)
     assert torch.equal(part[0], got[1])
+
+
+@pytest.mark.parametrize("N,V,out_in", [(1, 1 << 30, False)])
+def test_vocabularies_past_what_one_launch_counts(capi, N, V, out_in):
+    """The largest vocabulary, one feature: the logits of more tiles than a launch has threads for. With one feature z = x w is one
+    product, off by 2^-22 of it at most, and a probability by that times 2 |z| and 2^-20 besides (exponential, sum, quotient)."""
+    x, w, _, t = make(N, 1, V, out_in, False, 0.0, True, seed=62)
+    t[0] = V - 1
+    (loss, gx, gw, gb), saved = run(capi, x, w, None, t, out_in)
+    assert not capi.linear_softmax_cross_entropy_bad_label(saved)
+    X, flat, step = x.double(), w.view(-1), 1 << (22 if N > 1 else 26)
+    lse = torch.full((N,), -math.inf, device="cuda", dtype=torch.float64)
+    for v in range(0, V, step):
+        lse = torch.logaddexp(lse, torch.logsumexp(X * flat[v:v + step].double(), dim=1))
+    want = float((lse - X[:, 0] * flat[t].double()).mean())
+    top = float(X.abs().max()) * float(flat.abs().max())
+    assert abs(float(loss) - want) <= 2.0 ** -21 * top + 2.0 ** -20 * (1 + float(lse.abs().max()))
+    want_gx = torch.zeros(N, device="cuda", dtype=torch.float64)
+    grad = gw.view(-1)
+    for v in range(0, V, step):
+        part = flat[v:v + step].double()
+        d = torch.exp(X * part - lse[:, None])
+        bar = d * (2 * 2.0 ** -22 * top + 2.0 ** -20)
+        inside = (t >= v) & (t < v + step)
+        d[inside.nonzero()[:, 0], t[inside] - v] -= 1
+        want_gx += torch.mv(d, part)
+        for got, scale in ((grad, X), (gb, torch.ones_like(X))):
+            off = (got[v:v + step].double() - (d * scale).sum(0) / N).abs()
+            tol = (bar * scale.abs()).sum(0) / N + 2.0 ** -20 * (d * scale).abs().sum(0) / N + 2.0 ** -100
+            assert bool((off <= tol).all()), (v, float((off / tol).max()))
+    # sum_v d w: a sum of V terms p w, whose error relative to the sum of their magnitudes (at most max |w|) is that of p and of the sum
+    tol = float(flat.abs().max()) / N * (2 * 2.0 ** -22 * top + 2.0 ** -18)
+    assert bool(((gx[:, 0].double() - want_gx / N).abs() <= tol).all())
