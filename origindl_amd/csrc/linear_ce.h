@@ -57,14 +57,15 @@ __device__ inline float finite_top(float m2)
     return m2 == -INFINITY ? 0.f : m2;
 }
 
-// merges (m2, s) of two sets of logits. fmaxf drops NaN from the maxima, the sums keep it.
-__device__ inline void merge(float &m, float &s, float m_o, float s_o)
+// merges (m2, s) of two sets of logits. fmaxf drops NaN from the maxima, the sums keep it. S: float within a tile, double over
+// the tiles, of which a large vocabulary has millions
+template <class S>
+__device__ inline void merge(float &m, S &s, float m_o, S s_o)
 {
     const float top = fmaxf(m, m_o), sub = finite_top(top);
-    s = s * pow2(m - sub) + s_o * pow2(m_o - sub);
+    s = s * (S)pow2(m - sub) + s_o * (S)pow2(m_o - sub);
     m = top;
 }
-
 
 inline size_t aligned(size_t n)
 {

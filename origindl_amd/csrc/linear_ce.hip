@@ -275,14 +275,16 @@ __global__ __launch_bounds__(kBlock) void ce_join_kernel(const float *__restrict
                                                          int64_t tiles, int64_t n_pad, const Labels labels, float *__restrict__ row, double *block_loss,
                                                          int *block_count, float *saved)
 {
-    __shared__ float sm[16][kJoinRows], ss[16][kJoinRows];
+    __shared__ float sm[16][kJoinRows];
+    __shared__ double ss[16][kJoinRows];
     __shared__ int last;
     const int r = threadIdx.x % kJoinRows, g = threadIdx.x / kJoinRows;
     const int64_t n = (int64_t)blockIdx.x * kJoinRows + r;
-    float m = -INFINITY, s = 0.f;
+    float m = -INFINITY;
+    double s = 0.0;
 #pragma unroll 8
     for (int64_t t = g; t < tiles; t += 16)
-        merge(m, s, part_m[t * n_pad + n], part_s[t * n_pad + n]);
+        merge(m, s, part_m[t * n_pad + n], (double)part_s[t * n_pad + n]);
     sm[g][r] = m, ss[g][r] = s;
     __syncthreads();
     if (threadIdx.x < 64)
@@ -293,9 +295,9 @@ __global__ __launch_bounds__(kBlock) void ce_join_kernel(const float *__restrict
         {
             for (int i = 1; i < 16; ++i)
                 merge(m, s, sm[i][r], ss[i][r]);
-            row[2 * n] = m, row[2 * n + 1] = s;
+            row[2 * n] = m, row[2 * n + 1] = (float)s;
             if (labels(n) >= 0)
-                loss = kLn2 * (double)m + log((double)s) - (double)target[n], count = 1;
+                loss = kLn2 * (double)m + log(s) - (double)target[n], count = 1;
             else
                 bad = label_of(labels.t, labels.is64, n) != labels.ignore;
         }

@@ -138,7 +138,7 @@ def test_few_rows_over_a_vocabulary_in_several_pieces(capi, shape, out_in):
     assert torch.equal(part[0], got[1])
 
 
-@pytest.mark.parametrize("N,V,out_in", [(1, 1 << 30, False)])
+@pytest.mark.parametrize("N,V,out_in", [(1, 1 << 30, False), (200, (1 << 28) + 3, True)])
 def test_vocabularies_past_what_one_launch_counts(capi, N, V, out_in):
     """The largest vocabulary, one feature: the logits of more tiles than a launch has threads for. With one feature z = x w is one
     product, off by 2^-22 of it at most, and a probability by that times 2 |z| and 2^-20 besides (exponential, sum, quotient)."""
