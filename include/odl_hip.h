@@ -356,7 +356,7 @@ int odl_hip_softmax_ce_loss_grad_device(const float *x, const void *t, int idx_i
  * are three bfloat16 numbers instead, exact, and six products. Neither call synchronises or allocates; both can be captured.
  * forward: device_saved8[0] the loss, [1] (an int) nonzero if a label that is not ignore_index lies outside [0, V) — such a
  * row is left out like an ignored one, the caller decides when to look —, [2] the number of counted rows, the rest and
- * row_stats are for the backward pass: [N, 2] (base-2 logarithm of the row's largest exp(z), sum of exp(z) over that), and
+ * row_stats are for the backward pass: [N, 2] (the row's largest logit, the sum of exp(z - it)), and
  * behind them, with up to 256 rows whose logits are at most a quarter of the weights' size, the logits:
  * odl_hip_linear_softmax_ce_row_stats_floats(N, K, V) floats in all.
  * backward: gx[N,K], gw (w's layout), gb[V], each may be NULL; the upstream gradient is read from device_gy[0] (NULL: 1).

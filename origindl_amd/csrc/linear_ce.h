@@ -10,7 +10,6 @@ namespace linear_ce
 {
 constexpr int kBlock = 256;
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr double kLn2  = 0.69314718055994530942;
 constexpr float kDScale = 32768.f;  // d lies in [-1, 1]: two float16 numbers keep 2^-22 of an element, or 2^-40
 
 // saved[] — what the forward pass leaves for the backward pass and the caller
@@ -51,19 +50,26 @@ __device__ inline float pow2(float v)
     return __builtin_amdgcn_exp2f(v);
 }
 
-// what is subtracted before 2^v: with m2 = -inf (an empty set, or logits that are all -inf) nothing, and the powers are 0
-__device__ inline float finite_top(float m2)
+// e^(z - m). The difference first: a logit times log2(e) overflows from 2.4e38 on, and a mask may hold the type's lowest value.
+__device__ inline float exp_under(float z, float m)
 {
-    return m2 == -INFINITY ? 0.f : m2;
+    return pow2((z - m) * kLog2e);
 }
 
-// merges (m2, s) of two sets of logits. fmaxf drops NaN from the maxima, the sums keep it. S: float within a tile, double over
+// what is subtracted from logits whose maximum is m: with m = -inf (an empty set, or logits that are all -inf) nothing, and the
+// powers are 0
+__device__ inline float finite_top(float m)
+{
+    return m == -INFINITY ? 0.f : m;
+}
+
+// merges (maximum m, s = sum e^(z - m)) of two sets of logits. fmaxf drops NaN from the maxima, the sums keep it. S: float within a tile, double over
 // the tiles, of which a large vocabulary has millions
 template <class S>
 __device__ inline void merge(float &m, S &s, float m_o, S s_o)
 {
     const float top = fmaxf(m, m_o), sub = finite_top(top);
-    s = s * (S)pow2(m - sub) + s_o * (S)pow2(m_o - sub);
+    s = s * (S)exp_under(m, sub) + s_o * (S)exp_under(m_o, sub);
     m = top;
 }
 

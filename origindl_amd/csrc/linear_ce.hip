@@ -1,9 +1,9 @@
 // A linear layer and its softmax cross-entropy as one operator, forward and backward, for vocabularies whose logits are not
 // to be stored: z[n][v] = x[n].w[v] + b[v] exists only as accumulators.
 //
-//   forward   per 256 (128, 64) vocabulary entries and token: m2 = max z * log2(e) and s = sum 2^(z log2(e) - m2), formed in the
-//             product's epilogue; one launch joins them per token: loss_n = ln2 * m2 + ln(s) - z[n][t_n]
-//   backward  the vocabulary in pieces: the logits of a piece again, d = 2^(z log2(e) - m2) / s - [v = t_n] from the accumulators,
+//   forward   per 256 (128, 64) vocabulary entries and token: m = max z and s = sum e^(z - m), formed in the product's epilogue;
+//             one launch joins them per token: loss_n = m + ln(s) - z[n][t_n]
+//   backward  the vocabulary in pieces: the logits of a piece again, d = e^(z - m) / s - [v = t_n] from the accumulators,
 //             written as the operands of the two products that follow (rows of tokens for gx += d.w, rows of vocabulary for
 //             gw = d^T.x); the sums over tokens for gb come out of the same epilogue.
 //
@@ -239,19 +239,18 @@ struct StatsEpilogue
                     top = fmaxf(top, c[e]);
                 m = fmaxf(m, top);
             }
-            float m2 = m * kLog2e;
-            const float sub = finite_top(m2);
+            const float sub = finite_top(m);
 #pragma unroll
             for (int mi = 0; mi < T::MI; ++mi)
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    s += pow2(fmaf(acc[mi][ni][e], kLog2e, -sub));
-            const float m_o = __shfl_xor(m2, 32, 64), s_o = __shfl_xor(s, 32, 64);
-            merge(m2, s, m_o, s_o);
+                    s += exp_under(acc[mi][ni][e], sub);
+            const float m_o = __shfl_xor(m, 32, 64), s_o = __shfl_xor(s, 32, 64);
+            merge(m, s, m_o, s_o);
             if (t.lane < 32)
             {
                 const int col = (t.wn * T::NI + ni) * 32 + t.lane;
-                lm[t.wm * T::kCols + col] = m2, ls[t.wm * T::kCols + col] = s;
+                lm[t.wm * T::kCols + col] = m, ls[t.wm * T::kCols + col] = s;
             }
         }
         __syncthreads();
@@ -267,7 +266,7 @@ struct StatsEpilogue
     }
 };
 
-// Joins the partial maxima and sums of 16 tokens a workgroup, 16 threads a token; row[2n] = m2, row[2n + 1] = s; the mean loss
+// Joins the partial maxima and sums of 16 tokens a workgroup, 16 threads a token; row[2n] = m, row[2n + 1] = s; the mean loss
 // by the last workgroup to finish, which adds the workgroups' sums in their order.
 constexpr int kJoinRows = 16;
 
@@ -297,7 +296,7 @@ __global__ __launch_bounds__(kBlock) void ce_join_kernel(const float *__restrict
                 merge(m, s, sm[i][r], ss[i][r]);
             row[2 * n] = m, row[2 * n + 1] = (float)s;
             if (labels(n) >= 0)
-                loss = kLn2 * (double)m + log(s) - (double)target[n], count = 1;
+                loss = (double)m - (double)target[n] + log(s), count = 1;
             else
                 bad = label_of(labels.t, labels.is64, n) != labels.ignore;
         }
@@ -347,7 +346,7 @@ struct GradEpilogue
     {
         const float inv_x = 1.f / saved[kScaleX], inv_w = 1.f / saved[kScaleW];
         float *scratch = t.wave_scratch();
-        float m2[T::NI], inv_s[T::NI];
+        float m[T::NI], inv_s[T::NI];
         int64_t label[T::NI];
         bool counts[T::NI];
 #pragma unroll
@@ -356,7 +355,7 @@ struct GradEpilogue
             const int64_t n = t.col_block(ni) * 32 + (t.lane & 31);
             label[ni]  = labels(n);
             counts[ni] = label[ni] >= 0;
-            m2[ni]     = counts[ni] ? row[2 * n] : 0.f;
+            m[ni]      = counts[ni] ? row[2 * n] : 0.f;
             inv_s[ni]  = counts[ni] ? kDScale / row[2 * n + 1] : 0.f;
             label[ni] -= v0;
         }
@@ -375,7 +374,7 @@ struct GradEpilogue
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                 {
-                    float d = pow2(fmaf(c[e], kLog2e, -m2[ni])) * inv_s[ni];
+                    float d = exp_under(c[e], m[ni]) * inv_s[ni];
                     if (here && at == (e & 7) + 16 * (e >> 3))
                         d -= kDScale;
                     c[e] = counts[ni] ? d : 0.f;  // by selection: the logits of a row that does not count may be anything

@@ -342,27 +342,27 @@ struct RowsStatsEpilogue
                         target[n] = z[nb][e];
                     top = fmaxf(top, z[nb][e]);
                 }
-                float m2 = top * kLog2e, s = 0.f;
-                const float sub = finite_top(m2);
+                float s = 0.f;
+                const float sub = finite_top(top);
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    s += pow2(fmaf(z[nb][e], kLog2e, -sub));
-                const float m_o = __shfl_xor(m2, 32, 64), s_o = __shfl_xor(s, 32, 64);
-                merge(m2, s, m_o, s_o);
+                    s += exp_under(z[nb][e], sub);
+                const float top_o = __shfl_xor(top, 32, 64), s_o = __shfl_xor(s, 32, 64);
+                merge(top, s, top_o, s_o);
                 if (lane < 32)
-                    lm[m * NB * 32 + nb * 32 + lane] = m2, ls[m * NB * 32 + nb * 32 + lane] = s;
+                    lm[m * NB * 32 + nb * 32 + lane] = top, ls[m * NB * 32 + nb * 32 + lane] = s;
             }
         }
         __syncthreads();
         if (threadIdx.x < NB * 32)
         {
             const int n = threadIdx.x;
-            float m2 = lm[n], s = ls[n];
+            float top = lm[n], s = ls[n];
 #pragma unroll
             for (int i = 1; i < VB; ++i)
-                merge(m2, s, lm[i * NB * 32 + n], ls[i * NB * 32 + n]);
+                merge(top, s, lm[i * NB * 32 + n], ls[i * NB * 32 + n]);
             const int64_t at = tile * (blocks_n * 32) + nb0 * 32 + n;
-            part_m[at] = m2, part_s[at] = s;
+            part_m[at] = top, part_s[at] = s;
         }
     }
 };
@@ -394,7 +394,7 @@ struct RowsGradEpilogue
             {
                 const int64_t n = (nb0 + nb) * 32 + (lane & 31), label = labels(n);
                 const bool counts = label >= 0;
-                const float m2 = counts ? row[2 * n] : 0.f, inv = counts ? 1.f / row[2 * n + 1] : 0.f;
+                const float top = counts ? row[2 * n] : 0.f, inv = counts ? 1.f / row[2 * n + 1] : 0.f;
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                 {
@@ -403,7 +403,7 @@ struct RowsGradEpilogue
                     float d = 0.f;
                     if (counts && v < V)
                     {
-                        d = pow2(fmaf(z[nb][e] + bias[e], kLog2e, -m2)) * inv;
+                        d = exp_under(z[nb][e] + bias[e], top) * inv;
                         if (v == label - v0)
                             d -= 1.f;
                     }

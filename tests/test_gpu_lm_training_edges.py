@@ -169,3 +169,54 @@ def test_vocabularies_past_what_one_launch_counts(capi, N, V, out_in):
     # sum_v d w: a sum of V terms p w, whose error relative to the sum of their magnitudes (at most max |w|) is that of p and of the sum
     tol = float(flat.abs().max()) / N * (2 * 2.0 ** -22 * top + 2.0 ** -18)
     assert bool(((gx[:, 0].double() - want_gx / N).abs() <= tol).all())
+
+
+# --------------------------------------------------------------------------------------------------- masks and magnitudes
+LOWEST = torch.finfo(torch.float32).min
+
+
+@pytest.mark.parametrize("N,K,V", [(5, 40, 130), (300, 70, 1000), (9, 300, 21000), (130, 600, 10500)])
+def test_a_mask_of_the_lowest_value_that_leaves_nothing(capi, N, K, V):
+    """Every entry masked with the type's lowest value: x w is lost in it (|z| < 2^-25 of it), all entries are equal, the loss is the
+    logarithm of their number and the gradient 1 / their number. Entries at -inf beside them are no entries."""
+    x, w, b, t = make(N, K, V, False, True, 0.0, True, seed=71)
+    for gone in (0, V // 3):
+        b[:] = LOWEST
+        b[V - gone:] = -float("inf")
+        t %= V - gone
+        (loss, gx, gw, gb), _ = run(capi, x, w, b, t, False)
+        left = V - gone
+        assert abs(float(loss) - math.log(left)) <= 2.0 ** -20 * (1 + math.log(left))
+        d = torch.full((N, left), 1.0 / left, device="cuda", dtype=torch.float64)
+        d[torch.arange(N, device="cuda"), t] -= 1
+        d /= N
+        zeros = torch.zeros(N, V - left, device="cuda", dtype=torch.float64)
+        d, size = torch.cat([d, zeros], 1), torch.cat([d.abs(), zeros], 1)
+        # a probability is off by 2^-20 of itself, as an operand by 2^-40 besides; products are held to 1e-5 of their rows
+        e = size * 2.0 ** -20 + 2.0 ** -40 / N
+        for got, want, tol in ((gb, d.sum(0), e.sum(0)),
+                               (gx, d @ w.t().double(), e @ w.t().double().abs() + 1e-5 * d.norm(dim=1)[:, None] * w.double().norm(dim=1)),
+                               (gw, x.t().double() @ d, x.t().double().abs() @ e + 1e-5 * x.double().norm(dim=0)[:, None] * d.norm(dim=0))):
+            assert bool(((got.double() - want).abs() <= tol).all())
+        assert bool((gb[left:] == 0).all()) and bool((gw[:, left:] == 0).all())
+
+
+@pytest.mark.parametrize("N,K,V", [(6, 30, 200), (300, 64, 900), (6, 300, 21000)])
+def test_masks_that_leave_an_entry_and_logits_near_the_ends_of_the_range(capi, N, K, V):
+    x, w, b, t = make(N, K, V, True, True, 0.0, True, seed=72)
+    # all but one entry at the lowest value: it has the whole probability
+    b[:] = LOWEST
+    b[7] = 0.25
+    t[:] = 7
+    (loss, gx, gw, gb), _ = run(capi, x, w, b, t, True)
+    assert float(loss) == 0 and all(bool((g == 0).all()) for g in (gx, gw, gb))
+    # logits of 3e38 and of -3e38 side by side: their distance overflows, the probabilities are 1 and 0
+    b[:] = -3e38
+    b[3] = 3e38
+    t[:] = 3
+    (loss, gx, gw, gb), _ = run(capi, x, w, b, t, True)
+    assert float(loss) == 0 and all(bool((g == 0).all()) for g in (gx, gw, gb))
+    t[0] = 5
+    loss, _ = capi.linear_softmax_cross_entropy(x, w, b, t, w_out_in=True)
+    # (the entries are float32's neighbours of 3e38; the mean of one such distance and N - 1 zeros, rounded once)
+    assert float(loss) == float(np.float32((float(b[3]) - float(b[5])) / N))
