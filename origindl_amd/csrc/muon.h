@@ -148,6 +148,13 @@ __device__ inline double sum_of_parts(const double *sums, int parts, double *scr
     return s;
 }
 
+// what U is multiplied by to be X0 as an operand; a zero matrix stays one with eps = 0 too
+__device__ inline double operand_factor(double squares, double eps)
+{
+    const double norm = sqrt(squares) + eps;
+    return norm == 0.0 ? 0.0 : (double)kScale / norm;
+}
+
 // the matrices of one call: rows <= cols on the sides m, n; see muon.hip
 struct Settings
 {

@@ -78,7 +78,7 @@ __global__ __launch_bounds__(kBlock) void muon_prepare_kernel(const Matrices a, 
     __shared__ double part[4];
     const int z = blockIdx.z;
     r.base += z * batch_bytes, t.base += z * batch_bytes;
-    const auto factor = [&] { return (double)kScale / (sqrt(sum_of_parts<4>(sums + (int64_t)z * parts, parts, part)) + eps); };
+    const auto factor = [&] { return operand_factor(sum_of_parts<4>(sums + (int64_t)z * parts, parts, part), eps); };
     split_tile(UpdateAt{{a.g[z], a.buf[z], a.momentum, a.nesterov}, a.cols}, factor, a.rows, a.cols, (int64_t)blockIdx.y * 64, (int64_t)blockIdx.x * 64, r, t, tile);
 }
 

@@ -140,7 +140,7 @@ __global__ __launch_bounds__(MB == 4 ? 512 : 256, 2) void muon_slim_kernel(const
         float *tile = reinterpret_cast<float *>(lds + (MODE == kWhole ? kStrip : 0));  // [m][C + 1]
         double factor = 1.0, squares = 0.0;
         if constexpr (MODE == kFirst)
-            factor = (double)kScale / (sqrt(sum_of_parts<W>(s.sums + (int64_t)z * s.parts, s.parts, norm_parts)) + s.eps);
+            factor = operand_factor(sum_of_parts<W>(s.sums + (int64_t)z * s.parts, s.parts, norm_parts), s.eps);
         const Update u{s.a.g[z], s.a.buf[z], s.a.momentum, s.a.nesterov};
         const bool tall = s.a.rows > s.a.cols;
         const int64_t m = tall ? s.a.cols : s.a.rows, n = tall ? s.a.rows : s.a.cols, n0 = (int64_t)strip * C;
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(MB == 4 ? 512 : 256, 2) void muon_slim_kernel(const
 #pragma unroll
             for (int w = 1; w < W; ++w)
                 squares += norm_parts[w];
-            factor = (double)kScale / (sqrt(squares) + s.eps);
+            factor = operand_factor(squares, s.eps);
         }
         else
         {

@@ -220,3 +220,18 @@ def test_masks_that_leave_an_entry_and_logits_near_the_ends_of_the_range(capi, N
     loss, _ = capi.linear_softmax_cross_entropy(x, w, b, t, w_out_in=True)
     # (the entries are float32's neighbours of 3e38; the mean of one such distance and N - 1 zeros, rounded once)
     assert float(loss) == float(np.float32((float(b[3]) - float(b[5])) / N))
+
+
+@pytest.mark.parametrize("rows,cols", [(50, 60), (300, 90), (200, 5000), (1, 1)])
+def test_a_zero_matrix_gives_zeros_without_eps_too(capi, rows, cols):
+    zero = torch.zeros(rows, cols, device="cuda")
+    for eps in (0.0, 1e-7):
+        assert bool((capi.newton_schulz(zero, eps=eps) == 0).all())
+        p, buf = torch.randn(rows, cols, device="cuda", generator=gen(81)), zero.clone()
+        (new,) = capi.muon_step_multi([p], [zero], [buf], lr=0.1, eps=eps)
+        assert torch.equal(new, p) and bool((buf == 0).all())
+    # without eps the magnitude does not matter, down to float32's smallest numbers
+    g = torch.randn(rows, cols, device="cuda", generator=gen(82))
+    small = (g.double() * 2.0 ** -140).float()
+    got, want = capi.newton_schulz(small, eps=0.0), schulz64(small, eps=0.0)
+    assert float((got.double() - want).norm()) <= schulz_bar(5) * max(1.0, float(want.norm()))
