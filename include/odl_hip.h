@@ -353,7 +353,8 @@ int odl_hip_softmax_ce_loss_grad_device(const float *x, const void *t, int idx_i
  * log-likelihood and the gradient its derivative. Products are float32 in accuracy (each operand as two float16 numbers,
  * three products, float32 sums): an operand's elements are kept to 2^-22 of themselves, or to 2^-40 of the largest one where
  * that is more (the gradients' operand softmax - one-hot: to 2^-40). Up to 256 rows over 6 million weights or more the operands
- * are three bfloat16 numbers instead, exact, and six products. Neither call synchronises or allocates; both can be captured.
+ * are three bfloat16 numbers instead, exact (elements under 2^-110 to 2^-133), and six products. Neither call synchronises or
+ * allocates; both can be captured.
  * forward: device_saved8[0] the loss, [1] (an int) nonzero if a label that is not ignore_index lies outside [0, V) — such a
  * row is left out like an ignored one, the caller decides when to look —, [2] the number of counted rows, the rest and
  * row_stats are for the backward pass: [N, 2] (the row's largest logit, the sum of exp(z - it)), and

@@ -181,8 +181,19 @@ __global__ __launch_bounds__(kBlock) void ce_prepare_kernel(const PrepArgs a)
         a.bias[v] = v < a.vn ? (a.b ? a.b[a.v0 + v] : 0.f) : -INFINITY;
 }
 
+// what takes the operands' scales out of a logit, the smaller factor first: the other one alone may lift it out of range
+struct Unscale
+{
+    float first, second;
+    __device__ explicit Unscale(const float *saved)
+    {
+        const float x = 1.f / saved[kScaleX], w = 1.f / saved[kScaleW];
+        first = fminf(x, w), second = fmaxf(x, w);
+    }
+};
+
 // a lane's logits of one accumulator block, rows as to_columns leaves them
-__device__ inline void logits_of(f32x16 &c, float inv_x, float inv_w, const float *bias, int lane)
+__device__ inline void logits_of(f32x16 &c, const Unscale &by, const float *bias, int lane)
 {
     to_columns(c);
     const float *b = bias + (lane >> 5) * 8;
@@ -193,8 +204,8 @@ __device__ inline void logits_of(f32x16 &c, float inv_x, float inv_w, const floa
 #pragma unroll
         for (int e = 0; e < 4; ++e)
         {
-            c[8 * h + e]     = c[8 * h + e] * inv_x * inv_w + b0[e];
-            c[8 * h + 4 + e] = c[8 * h + 4 + e] * inv_x * inv_w + b1[e];
+            c[8 * h + e]     = c[8 * h + e] * by.first * by.second + b0[e];
+            c[8 * h + 4 + e] = c[8 * h + 4 + e] * by.first * by.second + b1[e];
         }
     }
 }
@@ -211,7 +222,7 @@ struct StatsEpilogue
     template <class T, class Acc>
     __device__ void operator()(const T &t, Acc &acc) const
     {
-        const float inv_x = 1.f / saved[kScaleX], inv_w = 1.f / saved[kScaleW];
+        const Unscale by(saved);
         float *lm = reinterpret_cast<float *>(t.lds), *ls = lm + T::kWavesM * T::kCols;
 #pragma unroll
         for (int ni = 0; ni < T::NI; ++ni)
@@ -224,7 +235,7 @@ struct StatsEpilogue
             {
                 const int64_t v = t.row_block(mi) * 32;
                 f32x16 &c = acc[mi][ni];
-                logits_of(c, inv_x, inv_w, bias + v, t.lane);
+                logits_of(c, by, bias + v, t.lane);
                 if (label >= v && label < v + 32)
                 {
                     const int at = (int)(label - v) - 8 * (t.lane >> 5);
@@ -344,7 +355,7 @@ struct GradEpilogue
     template <class T, class Acc>
     __device__ void operator()(const T &t, Acc &acc) const
     {
-        const float inv_x = 1.f / saved[kScaleX], inv_w = 1.f / saved[kScaleW];
+        const Unscale by(saved);
         float *scratch = t.wave_scratch();
         float m[T::NI], inv_s[T::NI];
         int64_t label[T::NI];
@@ -368,7 +379,7 @@ struct GradEpilogue
             for (int ni = 0; ni < T::NI; ++ni)
             {
                 f32x16 &c = acc[mi][ni];
-                logits_of(c, inv_x, inv_w, bias + vb * 32, t.lane);
+                logits_of(c, by, bias + vb * 32, t.lane);
                 const int at = (int)(label[ni] - vb * 32) - 8 * (t.lane >> 5);
                 const bool here = label[ni] >= vb * 32 && label[ni] < vb * 32 + 32;
 #pragma unroll
@@ -420,7 +431,7 @@ struct GradEpilogue
     }
 };
 
-// out[i][j] (+)= acc * factor, factor = gy / counted rows over the operands' scales
+// out[i][j] (+)= acc * gy / counted rows over the operands' scales. The mean is taken first: the rows' sum may be out of range.
 struct OutEpilogue
 {
     float *out;
@@ -433,7 +444,7 @@ struct OutEpilogue
     template <class T, class Acc>
     __device__ void operator()(const T &t, Acc &acc) const
     {
-        const float g = (gy ? *gy : 1.f) / fmaxf(saved[kCounted], 1.f), inv = 1.f / saved[scale] / kDScale;
+        const float g = (gy ? *gy : 1.f) / fmaxf(saved[kCounted], 1.f) / kDScale, inv = 1.f / saved[scale];
 #pragma unroll
         for (int mi = 0; mi < T::MI; ++mi)
 #pragma unroll
@@ -449,7 +460,7 @@ struct OutEpilogue
                     if (r < rows)
                     {
                         float *at = out + t.split * split_stride + r * ld + col;
-                        const float v = acc[mi][ni][e] * inv * g;
+                        const float v = acc[mi][ni][e] * g * inv;
                         *at = add ? *at + v : v;
                     }
                 }

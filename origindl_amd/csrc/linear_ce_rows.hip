@@ -9,8 +9,9 @@
 //              512 MB of it the vocabulary goes through in pieces, whose sums for gx add up.
 //
 // Mathematics. A float32 number is the sum of three bfloat16 numbers, its first, second and third eight bits, cut off without
-// rounding: exact. Of the nine products of two such sums the six of at least 2^-16 of the whole are formed by bfloat16 matrix
-// instructions (v_mfma_f32_32x32x16_bf16), exact in float32, and summed there: what is left out is under 2^-23 of |a||b|. No
+// rounding: exact (elements under 2^-110 to 2^-133, bfloat16's smallest number). Of the nine products of two such sums the six of
+// at least 2^-16 of the whole are formed by bfloat16 matrix instructions (v_mfma_f32_32x32x16_bf16), exact in float32, and summed
+// there: what is left out is under 2^-23 of |a||b|. No
 // scale is needed, as bfloat16 has float32's exponents, and so no pass over w to find one. Six products take 0.38 of the float32
 // matrix instruction's time. Measured: one row over 2048 x 32000, the forward pass streams 262 MB in 47 to 52 us (5.0 to 5.5
 // TB/s; a copy of 4 GiB reaches 4.8); over 2048 x 100000, forward and backward, 8 rows 692 us, 64 rows 875, 128 rows 1340,
@@ -367,8 +368,9 @@ struct RowsStatsEpilogue
     }
 };
 
-// d of a piece of the vocabulary, split: by_n as the small operand of gx, [V / 16][blocks of 32 rows]; by_v as an operand of gw, rows
-// of the vocabulary, [V / 32][rows / 16] (null: not wanted); and the sums over this workgroup's rows for gb
+// d / counted rows (the mean first: the rows' sum of d x may be out of range) of a piece of the vocabulary, split: by_n as the small
+// operand of gx, [V / 16][blocks of 32 rows]; by_v as an operand of gw, rows of the vocabulary, [V / 32][rows / 16] (null: not
+// wanted); and the sums over this workgroup's rows for gb
 struct RowsGradEpilogue
 {
     const float *b, *saved, *row;
@@ -382,6 +384,7 @@ struct RowsGradEpilogue
         constexpr int kTile = 32 * VB, kPitch = 32 * NB + 1;
         if (m < VB)
         {
+            const float share = 1.f / fmaxf(saved[kCounted], 1.f);
             float bias[16];
 #pragma unroll
             for (int e = 0; e < 16; ++e)
@@ -406,6 +409,7 @@ struct RowsGradEpilogue
                         d = exp_under(z[nb][e] + bias[e], top) * inv;
                         if (v == label - v0)
                             d -= 1.f;
+                        d *= share;
                     }
                     lds[at * kPitch + nb * 32 + (lane & 31)] = d;
                 }
@@ -503,7 +507,7 @@ struct RowsPartEpilogue
     }
 };
 
-__global__ __launch_bounds__(kBlock) void ce_rows_gb_kernel(const float *__restrict__ sums, int groups, int64_t V, const float *saved, const float *gy, float *__restrict__ gb)
+__global__ __launch_bounds__(kBlock) void ce_rows_gb_kernel(const float *__restrict__ sums, int groups, int64_t V, const float *gy, float *__restrict__ gb)
 {
     const int64_t v = (int64_t)blockIdx.x * kBlock + threadIdx.x;
     if (v >= V)
@@ -511,15 +515,15 @@ __global__ __launch_bounds__(kBlock) void ce_rows_gb_kernel(const float *__restr
     float s = sums[v * groups];
     for (int i = 1; i < groups; ++i)
         s += sums[v * groups + i];
-    gb[v] = s * ((gy ? *gy : 1.f) / fmaxf(saved[kCounted], 1.f));
+    gb[v] = gy ? s * *gy : s;
 }
 
-// gx[n][k] = factor * the runs' sums, in order; a workgroup takes 32 features and 32 rows
-__global__ __launch_bounds__(kBlock) void ce_rows_gx_kernel(const float *__restrict__ parts, int runs, int64_t N, int64_t K, int rows, const float *saved, const float *gy,
+// gx[n][k] = gy * the runs' sums, in order; a workgroup takes 32 features and 32 rows
+__global__ __launch_bounds__(kBlock) void ce_rows_gx_kernel(const float *__restrict__ parts, int runs, int64_t N, int64_t K, int rows, const float *gy,
                                                             float *__restrict__ gx)
 {
     __shared__ float tile[32][33];
-    const float g = (gy ? *gy : 1.f) / fmaxf(saved[kCounted], 1.f);
+    const float g = gy ? *gy : 1.f;
     const int64_t k0 = (int64_t)blockIdx.x * 32, n0 = (int64_t)blockIdx.y * 32;
     for (int i = threadIdx.x; i < 32 * 32; i += kBlock)
     {
@@ -540,13 +544,13 @@ __global__ __launch_bounds__(kBlock) void ce_rows_gx_kernel(const float *__restr
     }
 }
 
-// gw = factor * d^T.x over the rows: out[r][c] from operands split by r and by c, [blocks of 32][rows / 16]. A wave makes 32 rows of 128
+// gw = gy * d^T.x over the rows: out[r][c] from operands split by r and by c, [blocks of 32][rows / 16]. A wave makes 32 rows of 128
 // columns; the four waves of a workgroup share the columns' operand, and walk down `steps` blocks of 128 rows.
 __global__ __launch_bounds__(kBlock, 2) void ce_rows_outer_kernel(const u32x4 *__restrict__ by_r, const u32x4 *__restrict__ by_c, int kbs, int64_t rows, int64_t cols, int64_t ld,
-                                                                  unsigned tiles_c, int steps, const float *saved, const float *gy, float *__restrict__ out)
+                                                                  unsigned tiles_c, int steps, const float *gy, float *__restrict__ out)
 {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const float g = (gy ? *gy : 1.f) / fmaxf(saved[kCounted], 1.f);
+    const float g = gy ? *gy : 1.f;
     const unsigned group = blockIdx.x / tiles_c;
     const int64_t c0 = (int64_t)(blockIdx.x - group * tiles_c) * 128;
     for (int step = 0; step < steps; ++step)
@@ -789,7 +793,7 @@ int few_backward(const Problem &p, const float *gy, const float *saved, const fl
             return rc;
         if (gb)
         {
-            ce_rows_gb_kernel<<<dim3((unsigned)ceil_div(vn, kBlock)), dim3(kBlock), 0, st>>>(s.sums, blocks_n / taken_of(blocks_n), vn, saved, gy, gb + v0);
+            ce_rows_gb_kernel<<<dim3((unsigned)ceil_div(vn, kBlock)), dim3(kBlock), 0, st>>>(s.sums, blocks_n / taken_of(blocks_n), vn, gy, gb + v0);
             ODL_LAUNCH_CHECK();
         }
         if (gx)
@@ -805,13 +809,13 @@ int few_backward(const Problem &p, const float *gy, const float *saved, const fl
             if (int rc = check_blocks(blocks, kBlock))
                 return rc;
             ce_rows_outer_kernel<<<dim3((unsigned)blocks), dim3(kBlock), 0, st>>>(p.w_out_in ? s.d_by_v : s.x_by_k, p.w_out_in ? s.x_by_k : s.d_by_v,
-                                                                                 blocks_n * 2, r, c, ld, (unsigned)tiles_c, steps, saved, gy, gw + at);
+                                                                                 blocks_n * 2, r, c, ld, (unsigned)tiles_c, steps, gy, gw + at);
             ODL_LAUNCH_CHECK();
         }
     }
     if (gx)
     {
-        ce_rows_gx_kernel<<<dim3((unsigned)ceil_div(p.K, 32), (unsigned)blocks_n), dim3(kBlock), 0, st>>>(s.parts, runs, p.N, p.K, blocks_n * 32, saved, gy, gx);
+        ce_rows_gx_kernel<<<dim3((unsigned)ceil_div(p.K, 32), (unsigned)blocks_n), dim3(kBlock), 0, st>>>(s.parts, runs, p.N, p.K, blocks_n * 32, gy, gx);
         ODL_LAUNCH_CHECK();
     }
     return ODL_OK;

@@ -235,3 +235,35 @@ def test_a_zero_matrix_gives_zeros_without_eps_too(capi, rows, cols):
     small = (g.double() * 2.0 ** -140).float()
     got, want = capi.newton_schulz(small, eps=0.0), schulz64(small, eps=0.0)
     assert float((got.double() - want).norm()) <= schulz_bar(5) * max(1.0, float(want.norm()))
+
+
+@pytest.mark.parametrize("N,K,V", [(50, 70, 200), (300, 70, 200), (50, 31000, 200)])
+@pytest.mark.parametrize("sx,sw", [(1e35, 1e-32), (1e-32, 1e35), (3e36, 1e-36)])
+def test_operands_of_opposite_magnitudes(capi, N, K, V, sx, sw):
+    """Logits up to thousands from operands near the ends of float32's range. Few rows over large weights: an operand's three bfloat16
+    parts end at bfloat16's smallest number, 2^-133, so an element is off by that at most and a logit by 2^-133 (|x|_1 + |w|_1): of
+    weights about 1e-38 that is their seventh bit, and the bars are widened by it."""
+    x, w, b, t = make(N, K, V, False, True, 0.0, True, seed=91)
+    x, w = x * sx, w * sw
+    got, _ = run(capi, x, w, b, t, False)
+    want, bars = definition(x, w, b, t, False)
+    if N * K >= 50 * 31000:
+        e = 2.0 ** -133 * float(x.double().abs().sum(1).max() + w.double().abs().sum(0).max())
+        lift = math.expm1(2 * e)  # of a probability, in each gradient: softmax - one-hot is off by lift * p, |p| <= 1
+        W, X = w.t().double(), x.double()
+        bars = (bars[0] + 2 * e, bars[1] + lift * W.abs().max(dim=0).values / N, bars[2] + lift * X.abs().sum(0)[:, None] / N, bars[3] + lift)
+    check(got, want, bars)
+    assert all(bool(g.isfinite().all()) for g in got)
+
+
+@pytest.mark.parametrize("N,K,V", [(300, 8, 2), (250, 8, 750001), (70, 2000, 3001)])
+def test_a_mean_gradient_whose_sum_is_out_of_range(capi, N, K, V):
+    """Rows of 1e37 to 2e37 under one label: the sum over the rows overflows, the mean does not."""
+    g = gen(92)
+    x = (1 + torch.rand(N, K, device="cuda", generator=g)) * 1e37
+    w, b = torch.zeros(V, K, device="cuda"), torch.zeros(V, device="cuda")
+    t = torch.zeros(N, dtype=torch.long, device="cuda")
+    got, _ = run(capi, x, w, b, t, True)
+    want, bars = definition(x, w, b, t, True)
+    check(got, want, bars)
+    assert bool(got[2].isfinite().all())
