@@ -119,10 +119,11 @@ __device__ inline void load_fragment(const Panel &p, int64_t rb, int64_t kb, int
 }
 
 // 16 bytes a lane from a buffer into LDS: lane i's data lands at lds_byte_address + 16 * i. An instruction and not the
-// compiler's builtin, which would wait for all queued loads before every LDS read; the waits are placed by hand.
+// compiler's builtin, which would wait for all queued loads before every LDS read; the waits are placed by hand. (One wait
+// state between the write of m0 and the load that reads it: inside the asm the compiler does not add it.)
 __device__ inline void load_to_lds_16(i32x4 rsrc, unsigned lds_byte_address, unsigned lane_offset, unsigned offset)
 {
-    asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  :
                  : "s"(lds_byte_address), "v"(lane_offset), "s"(rsrc), "s"(offset)
                  : "memory", "m0");
