@@ -350,9 +350,11 @@ int odl_hip_softmax_ce_loss_grad_device(const float *x, const void *t, int idx_i
  * Rows whose label is ignore_index are not counted (pass a value no label has, e.g. -100, to count all): they add nothing to
  * the loss or to a gradient, whatever x holds there, NaN included. With no counted row the loss and all gradients are 0.
  * Unlike odl_hip_softmax_ce_loss the probability is not offset by 1e-8 before the logarithm: the loss is the exact negative
- * log-likelihood and the gradient its derivative. Products are float32 in accuracy (each operand as two float16 numbers,
- * three products, float32 sums): an operand's elements are kept to 2^-22 of themselves, or to 2^-40 of the largest one where
- * that is more (the gradients' operand softmax - one-hot: to 2^-40). Up to 256 rows over 6 million weights or more the operands
+ * log-likelihood and the gradient its derivative. Each operand of a product is two float16 numbers, a product three of theirs,
+ * sums are float32: as accurate as a float32 product where an operand's elements lie within 2^17 of its largest. Elements are
+ * kept to 2^-22 of themselves, to 2^-39 of the largest one (x: of the counted rows) or to 2^-145, whichever is most, so a row
+ * far smaller than the largest loses digits; the gradients' operand softmax - one-hot is kept to 2^-40, so an entry of
+ * probability under 2^-41 has no gradient. Up to 256 rows over 6 million weights or more the operands
  * are three bfloat16 numbers instead, exact (elements under 2^-110 to 2^-133), and six products. Neither call synchronises or
  * allocates; both can be captured.
  * forward: device_saved8[0] the loss, [1] (an int) nonzero if a label that is not ignore_index lies outside [0, V) — such a
@@ -665,8 +667,8 @@ int odl_hip_sgd_step_multi_decay(int count, const float *const *p, float *const 
 /* Orthogonalised updates, for a matrix optimiser beside SGD and Adam (no counterpart in the reference).
  * newton_schulz: out = X after `steps` of X <- a X + (b A + c A A) X, A = X X^T, from X0 = g / (||g||_F + eps), on the side of
  * the shorter dimension, for `batch` dense matrices g[batch, rows, cols]. (a, b, c) = (3.4445, -4.775, 2.0315) brings the
- * singular values to about [0.7, 1.2] in five steps. Coefficients under which they, or b A + c A A, could pass 7.5 on the way
- * are refused. Elements of X are kept to 2^-22 of themselves or 2^-38. A zero matrix gives zeros; a matrix with an infinity or
+ * singular values to about [0.7, 1.2] in five steps. Coefficients under which they could pass 2.73 on the way (A, their
+ * squares: 7.5), or b A + c A A could pass 7.5, are refused. Elements of X are kept to 2^-22 of themselves or 2^-38. A zero matrix gives zeros; a matrix with an infinity or
  * a NaN gives NaN. out may be g.
  * muon_step_multi: one optimiser step over a list of matrices [host_rows[i], host_cols[i]]; equal shapes go through the same
  * launches, up to 32 together:
@@ -674,7 +676,8 @@ int odl_hip_sgd_step_multi_decay(int count, const float *const *p, float *const 
  *   p_out = p * (1 - lr * weight_decay) - lr * sqrt(max(1, outputs / inputs)) * O
  * A matrix is [outputs, inputs] (a convolution's filters as [OC, the rest], LinearOp's weight); with host_in_out[i] != 0 in
  * muon_step_multi_in_out entry i is [inputs, outputs], as nn::Linear keeps its weight (host_in_out null: none is).
- * buf is updated in place, p_out may be p; a buf or a p_out that stands for two entries is refused. Empty matrices are skipped.
+ * buf is updated in place, p_out may be p and must overlap no other operand, buf none; a buf or a p_out that stands for two
+ * entries is refused. Empty matrices are skipped.
  * Sides up to 2^20, 1 to 100 steps. Neither call synchronises or allocates device memory; both can be captured. */
 int odl_hip_newton_schulz(const float *g, int64_t batch, int64_t rows, int64_t cols, int steps, float a, float b, float c,
                           float eps, float *out, void *workspace, size_t workspace_bytes, void *stream);

@@ -101,10 +101,13 @@ struct Problem
 };
 
 // Few rows over large weights: the bytes of the weights are what a pass costs, and they are read as they lie, no operand laid out
-// first. Measured with one row over 2048 x 32000: forward 61 us against 306; over 2048 x 100000, forward and backward, 64 rows
-// 875 us against 1364, 128 rows 1340 against 2503. A tile of the streams holds 32, 64 or 128 rows, and a part of one costs the
-// whole. With 64 rows over 256 x 1000 the operands laid out win, 68 us against 98: their launches fill the chip where the
-// streams' tiles of 128 entries do not. The estimates of both cross at about 6 million weights.
+// first. Measured in us, weights [K, V], streams against operands laid out: one row over 2048 x 32000, forward, 61 and 231;
+// forward and backward over 2048 x 100000 64 rows 877 and 1930, 128 rows 1343 and 2232, 256 rows 2314 and 2570. A tile of the
+// streams holds 32, 64 or 128 rows, and a part of one costs the whole: under 6 million weights operands laid out win from 65 rows
+// on (1024 x 4000: 80 rows 94 and 86, 256 rows 113 and 95; up to 64 rows the streams are up to a quarter faster there as well).
+// The rule does not look at the weights' shape. Narrow ones, which d outweighs, would be faster laid out from 65 rows on (64 x 128000:
+// 128 rows 331 and 176, 64 rows 178 and 161; 256 x 32000: 128 rows 154 and 114), and so would short vocabularies, whose few tiles
+// leave compute units idle (7000 x 900: 128 rows 215 and 189).
 inline bool few_rows(int64_t N, int64_t K, int64_t V)
 {
     return N <= 256 && K * V >= 6000000;

@@ -83,7 +83,8 @@ __global__ __launch_bounds__(kBlock) void ce_magnitudes_kernel(const float *__re
         reinterpret_cast<int *>(saved)[kTicket] = 0;
 }
 
-// the power of two that brings magnitude m to [2^14, 2^15): float16 holds it, and what is 2^18 times smaller keeps its bits
+// the power of two that brings magnitude m to [2^14, 2^15): float16 holds it, and what is 2^17 times smaller keeps its bits (a
+// largest magnitude under 2^-106 is brought less far, its operand's elements are kept to 2^-145)
 __device__ inline float scale_for(float m)
 {
     if (!(m > 0.f))

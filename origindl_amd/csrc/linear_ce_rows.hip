@@ -11,11 +11,11 @@
 // Mathematics. A float32 number is the sum of three bfloat16 numbers, its first, second and third eight bits, cut off without
 // rounding: exact (elements under 2^-110 to 2^-133, bfloat16's smallest number). Of the nine products of two such sums the six of
 // at least 2^-16 of the whole are formed by bfloat16 matrix instructions (v_mfma_f32_32x32x16_bf16), exact in float32, and summed
-// there: what is left out is under 2^-23 of |a||b|. No
-// scale is needed, as bfloat16 has float32's exponents, and so no pass over w to find one. Six products take 0.38 of the float32
-// matrix instruction's time. Measured: one row over 2048 x 32000, the forward pass streams 262 MB in 47 to 52 us (5.0 to 5.5
-// TB/s; a copy of 4 GiB reaches 4.8); over 2048 x 100000, forward and backward, 8 rows 692 us, 64 rows 875, 128 rows 1340,
-// 256 rows 2346: past 64 rows the splitting and the products take longer than the bytes.
+// there: what is left out is under 2^-23 of |a||b|. No scale is needed, as bfloat16 has float32's exponents, and so no pass over w
+// to find one. Six products take 0.38 of the float32 matrix instruction's time. Measured: one row over 2048 x 32000, weights
+// [K, V], the forward pass streams 262 MB in 47 to 52 us (5.0 to 5.5 TB/s; a copy of 4 GiB reaches 4.8); over 2048 x 100000, [K, V] and
+// [V, K], forward and backward, 8 rows 700 and 735 us, 64 rows 877 and 895, 128 rows 1343 and 1360, 256 rows 2314 and 2350: past
+// 64 rows the splitting and the products take longer than the bytes.
 //
 // Both products with w are one kernel: w is [out][contraction] for the logits of a [V, K] weight and [contraction][out] for its
 // gx, and the other way round for a [K, V] weight. Eight waves share a tile of outputs, each takes an eighth of the contraction,

@@ -16,7 +16,8 @@
 // sizes takes 10 to 12 us, its operations alone 3).
 //
 // Singular values of X stay under max |f| on [0, 1], f(s) = a s + b s^3 + c s^5 (1.21 for the usual coefficients), so all
-// operands are scaled by the same 2^13: float16 holds 8 * 2^13, and coefficients that lead past 7.5 are refused.
+// operands are scaled by the same 2^13: float16 holds 8 * 2^13, and coefficients that lead A = X X^T (the singular values'
+// squares) or b A + c A A past 7.5 are refused.
 #include <cmath>
 
 #include "muon.h"

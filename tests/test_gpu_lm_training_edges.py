@@ -267,3 +267,14 @@ def test_a_mean_gradient_whose_sum_is_out_of_range(capi, N, K, V):
     want, bars = definition(x, w, b, t, True)
     check(got, want, bars)
     assert bool(got[2].isfinite().all())
+
+
+@pytest.mark.parametrize("N,K,V", [(300, 256, 700), (64, 3000, 2100)])
+def test_rows_and_entries_of_unequal_size(capi, N, K, V):
+    """Rows of x, and entries of w, from 1 down to 2^-24 of the largest: each row's logits keep the bar of a float32 product of its own
+    row (an element is off by 2^-39 of the largest, 2^-15 of an element 2^-24 as large, and those errors add up as a sum's)."""
+    x, w, b, t = make(N, K, V, True, True, 0.1, True, seed=95)
+    x = x * torch.logspace(0, -24, N, base=2, device="cuda")[torch.randperm(N, device="cuda", generator=gen(96))][:, None]
+    w = w * torch.logspace(0, -24, V, base=2, device="cuda")[torch.randperm(V, device="cuda", generator=gen(97))][:, None]
+    got, _ = run(capi, x, w, b, t, True)
+    check(got, *definition(x, w, b, t, True))
