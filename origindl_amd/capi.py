@@ -510,7 +510,7 @@ def _ce_args(who, x, w, b, t, w_out_in):
     V, Kw = w.shape if w_out_in else (w.shape[1], w.shape[0])
     if K != Kw:
         raise OdlInvalidArgument("%s: x has %d features, w expects %d" % (who, K, Kw))
-    if b is not None and (_chk(b, "b").numel() != V or b.shape[-1] != V):
+    if b is not None and (_chk(b, "b").numel() != V or b.dim() == 0 or b.shape[-1] != V):
         raise OdlInvalidArgument("%s: b must hold %d values, got shape %s" % (who, V, tuple(b.shape)))
     t, is64 = _labels(t)
     if t.dim() != 1 or t.shape[0] != N:

@@ -7,7 +7,7 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_lm_training import COEF, check, definition, gen, make, muon64, run, schulz64, schulz_bar
+from test_gpu_lm_training import COEF, check, definition, gen, make, run, schulz64, schulz_bar
 
 pytestmark = pytest.mark.gpu
 
@@ -278,3 +278,11 @@ def test_rows_and_entries_of_unequal_size(capi, N, K, V):
     w = w * torch.logspace(0, -24, V, base=2, device="cuda")[torch.randperm(V, device="cuda", generator=gen(97))][:, None]
     got, _ = run(capi, x, w, b, t, True)
     check(got, *definition(x, w, b, t, True))
+
+
+def test_a_bias_without_dimensions_is_refused(capi):
+    x, w, _, t = make(4, 8, 1, False, False, 0.0, True, seed=98)
+    with pytest.raises(capi.OdlInvalidArgument):
+        capi.linear_softmax_cross_entropy(x, w, torch.zeros((), device="cuda"), t)
+    loss, _ = capi.linear_softmax_cross_entropy(x, w, torch.zeros(1, device="cuda"), t)
+    assert float(loss) == 0  # one class: its probability is 1
