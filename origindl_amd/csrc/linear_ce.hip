@@ -286,8 +286,8 @@ __global__ __launch_bounds__(kBlock) void ce_join_kernel(const float *__restrict
                                                          int64_t tiles, int64_t n_pad, const Labels labels, float *__restrict__ row, double *block_loss,
                                                          int *block_count, float *saved)
 {
-    __shared__ float sm[16][kJoinRows];
-    __shared__ double ss[16][kJoinRows];
+    __shared__ float sm[4][kJoinRows];
+    __shared__ double ss[4][kJoinRows];
     __shared__ int last;
     const int r = threadIdx.x % kJoinRows, g = threadIdx.x / kJoinRows;
     const int64_t n = (int64_t)blockIdx.x * kJoinRows + r;
@@ -296,7 +296,16 @@ __global__ __launch_bounds__(kBlock) void ce_join_kernel(const float *__restrict
 #pragma unroll 8
     for (int64_t t = g; t < tiles; t += 16)
         merge(m, s, part_m[t * n_pad + n], (double)part_s[t * n_pad + n]);
-    sm[g][r] = m, ss[g][r] = s;
+    // a wave's four threads of a token, then the four waves
+#pragma unroll
+    for (int o = kJoinRows; o < 64; o *= 2)
+    {
+        const float m_o  = __shfl_xor(m, o, 64);
+        const double s_o = __shfl_xor(s, o, 64);
+        merge(m, s, m_o, s_o);
+    }
+    if ((threadIdx.x & 63) < kJoinRows)
+        sm[threadIdx.x >> 6][r] = m, ss[threadIdx.x >> 6][r] = s;
     __syncthreads();
     if (threadIdx.x < 64)
     {
@@ -304,7 +313,8 @@ __global__ __launch_bounds__(kBlock) void ce_join_kernel(const float *__restrict
         int count = 0, bad = 0;
         if (threadIdx.x < kJoinRows && n < labels.N)
         {
-            for (int i = 1; i < 16; ++i)
+#pragma unroll
+            for (int i = 1; i < 4; ++i)
                 merge(m, s, sm[i][r], ss[i][r]);
             row[2 * n] = m, row[2 * n + 1] = (float)s;
             if (labels(n) >= 0)
