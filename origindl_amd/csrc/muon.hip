@@ -11,9 +11,9 @@
 // as rows of m (for X X^T) and as rows of n (for B X), the symmetric ones with their mirror image. The last one writes X, or
 // applies it to the parameter.
 //
-// Measured: 4096 x 4096, five steps: 4.0 ms, 341 TFLOP/s of the work that symmetry leaves (the chip's power limit for these
-// products is 425 to 455); 1024 x 1024: 173 us, seventeen launches of which each waits for the one before (a product of these
-// sizes takes 10 to 12 us, its operations alone 3).
+// Measured: 4096 x 4096, five steps: 4.0 to 4.15 ms, 331 to 343 TFLOP/s of the work that symmetry leaves (the chip's power limit
+// for these products is 425 to 455); 1000 x 1000: 172 us, seventeen launches of which each waits for the one before (a product of
+// these sizes takes 10 to 12 us, its operations alone 3).
 //
 // Singular values of X stay under max |f| on [0, 1], f(s) = a s + b s^3 + c s^5 (1.21 for the usual coefficients), so all
 // operands are scaled by the same 2^13: float16 holds 8 * 2^13, and coefficients that lead A = X X^T (the singular values'
