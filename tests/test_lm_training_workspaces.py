@@ -36,7 +36,7 @@ def group_of(count, rows, cols):
     return max(1, min(count, KGROUP, GROUP_BYTES // (16 * m * n + 8 * m * m)))
 
 
-SIDES = (40, 128, 200, 256, 320, 384, 512, 640, 768, 1000, 1024, 1536, 1920, 2048, 2560, 3072, 4096, 6000, 8192, 11008, 16384, 50000)
+SIDES = (40, 128, 200, 256, 320, 384, 512, 640, 768, 1000, 1024, 1536, 1920, 2048, 2560, 3000, 4096, 6000, 8192, 11008, 16384, 50000)
 
 
 @pytest.mark.parametrize("rows", SIDES)
@@ -57,7 +57,7 @@ def test_a_batch_asks_for_what_each_of_its_groups_needs(l, rows):
 
 
 def test_shapes_whose_last_group_needs_the_most(l):
-    for count, rows, cols, rest in ((63, 384, 1920, 31), (61, 512, 3072, 29), (62, 512, 4096, 30), (63, 512, 4096, 31)):
+    for count, rows, cols, rest in ((63, 384, 1920, 31), (63, 320, 1920, 31), (62, 512, 4096, 30), (63, 512, 4096, 31)):
         assert schulz(l, rest, rows, cols) > schulz(l, 32, rows, cols)
         assert schulz(l, count, rows, cols) == muon(l, count, rows, cols) == schulz(l, rest, rows, cols)
 
